@@ -509,6 +509,117 @@ TL_API tl_status tl_lmhead_argmax_noalloc(const float* x, const float* gamma, fl
                                           int32_t hidden, int32_t* token_out, float* logits_out,
                                           void* stream);
 
+/* ------------------------------------------------- paged KV cache (serving)
+ * A pool of fixed-size pages shared by all sequences, for callers that drive
+ * their own batch (the engine above keeps one contiguous slot per sequence).
+ * No counterpart in the reference, whose cache is one region per run
+ * (rtl/memory/kv_cache_manager.sv:43-47).
+ *
+ * Element types of the operators below. */
+typedef enum tl_dtype { TL_F32 = 0, TL_BF16 = 1, TL_F16 = 2, TL_I8 = 3 } tl_dtype;
+
+/* One layer's pool, device memory: k and v are [num_pages][kv_heads][page_size][head_dim]
+ * of TL_I8, TL_BF16 or TL_F16, contiguous and 16-byte aligned; a TL_I8 pool
+ * has one float32 scale per stored row, k_scale and v_scale
+ * [num_pages][kv_heads][page_size] (row = int8 * scale; quantize_int8,
+ * model/tinyllama_gemm_int8.py:36-42, applied to each row by itself).
+ * head_dim is 64 or 128; page_size is any positive number. */
+typedef struct tl_paged_kv {
+  void* k;
+  void* v;
+  float* k_scale;  /* TL_I8 only */
+  float* v_scale;
+  int32_t dtype;   /* tl_dtype */
+  int32_t num_pages;
+  int32_t kv_heads;
+  int32_t page_size;
+  int32_t head_dim;
+} tl_paged_kv;
+
+/* How the operators find a row: position p of sequence s is row p % page_size
+ * of page block_table[s * table_stride + p / page_size], with block_table
+ * int32 [n_seqs][max_pages] on the device (table_stride >= max_pages). The
+ * contents of block_table, seq, pos and lengths are device data that no call
+ * reads on the host: an entry that names no sequence (outside [0, n_seqs)), no
+ * position (outside [0, max_pages * page_size)) or no page (outside
+ * [0, num_pages)) names no row. Such rows are never read or written, and each
+ * operator says what it gives for them. A batch of fixed size is padded with
+ * seq = -1.
+ *
+ * Activations (q, k, v) are [rows][heads][head_dim] of TL_F32, TL_BF16 or
+ * TL_F16, head rows contiguous, token rows *_stride elements apart (so q, k
+ * and v can be columns of one fused projection); base and row stride are
+ * multiples of 16 bytes. All pointers are device pointers. */
+
+/* Appends `tokens` key and value rows (k, v [tokens][kv_heads][head_dim]) at
+ * (seq[t], pos[t]), keys rotated by their position on the way: with cos/sin
+ * float32 [max_positions][head_dim] (rope_cos/rope_sin above; only the first
+ * head_dim / 2 columns are read, the second half repeats them), element j and
+ * j + head_dim/2 turn as a' = a cos - b sin, b' = b cos + a sin in float32
+ * without contraction (model/tinyllama.py:59-80), then round once
+ * to the pool's type. q (may be NULL, else [tokens][heads][head_dim]) is
+ * rotated in the same way into q_out [tokens][heads][head_dim], contiguous, of
+ * the same type (q_out == q for contiguous q rotates in place). Tokens that
+ * name no row write nothing to the pool; a position outside [0, max_positions)
+ * has no angle: nothing is stored and its q_out row is zero. cos == sin ==
+ * NULL stores keys as they are (q must be NULL): rows that tl_paged_read gave
+ * from another pool. Two tokens of a call must not name one row. A row with an
+ * infinity or a NaN gets a NaN scale in a TL_I8 pool. */
+TL_API tl_status tl_paged_append(const tl_paged_kv* cache, const void* q, const void* k, const void* v, int32_t dtype,
+                                 int64_t q_stride, int64_t k_stride, int64_t v_stride, const int32_t* seq,
+                                 const int32_t* pos, const int32_t* block_table, int32_t n_seqs, int32_t max_pages,
+                                 int64_t table_stride, const float* rope_cos, const float* rope_sin,
+                                 int32_t max_positions, int32_t tokens, int32_t heads, void* q_out, void* stream);
+
+/* Reads rows (seq[t], pos[t]) back into k_out, v_out [tokens][kv_heads][head_dim]
+ * of out_dtype (TL_F32, TL_BF16 or TL_F16), contiguous, 16-byte aligned,
+ * rounded once; either may be NULL. Tokens that name no row give zeros. */
+TL_API tl_status tl_paged_read(const tl_paged_kv* cache, const int32_t* seq, const int32_t* pos,
+                               const int32_t* block_table, int32_t n_seqs, int32_t max_pages, int64_t table_stride,
+                               int32_t tokens, void* k_out, void* v_out, int32_t out_dtype, void* stream);
+
+/* Attention of one new token of each of `rows` sequences over the pool: for
+ * row r and query head h (kv head h / (heads / kv_heads)) over positions
+ * j < lengths[r] of sequence seq[r] (seq NULL: sequence r),
+ *   s_j = sm_scale * q[r][h] . k_j,  out[r][h] = sum_j softmax(s)_j v_j,
+ *   lse[r][h] = log sum_j exp(s_j)
+ * with q already rotated and the row's own key and value already appended.
+ * out [rows][heads][head_dim] has q's type and is contiguous; lse (float32
+ * [rows][heads]) may be NULL. Lengths beyond the table are cut to it;
+ * positions whose page does not exist are left out; a row without positions
+ * (length 0, padding) gives zeros and lse = -infinity. heads may be any
+ * multiple of kv_heads. Sums and softmax statistics are float32; products run
+ * on the tensor cores with the query and the probabilities split so that a
+ * float32 query keeps float32 accuracy for every pool type.
+ * workspace: tl_paged_attn_workspace_bytes bytes of device memory, 16-byte aligned, zeroed once
+ * by the caller before its first call; every call leaves it ready for the
+ * next. Calls that share one workspace must not overlap on the GPU. The call
+ * allocates nothing, does not synchronise and can be captured in a graph. */
+TL_API size_t tl_paged_attn_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t head_dim);
+TL_API tl_status tl_paged_attn_decode(const tl_paged_kv* cache, const void* q, int32_t q_dtype, int64_t q_stride,
+                                      const int32_t* seq, const int32_t* lengths, const int32_t* block_table,
+                                      int32_t n_seqs, int32_t max_pages, int64_t table_stride, int32_t rows,
+                                      int32_t heads, float sm_scale, void* out, float* lse, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* Log probabilities of given tokens, entropy and the top_k most likely tokens
+ * of each row of logits [rows][vocab] (TL_F32, TL_BF16 or TL_F16; rows
+ * row_stride elements apart, any alignment of the element type):
+ *   logprob[r]  = x[tokens[r]] - log sum exp x     (tokens NULL: not written)
+ *   entropy[r]  = -sum p log p, p = softmax(x)     (may be NULL)
+ *   top_ids[r][k], top_logprobs[r][k], k < top_k <= TL_TOP_K_MAX, the largest
+ *   first, equal logits by the lowest id (argmax_reduction.sv:47-58).
+ * A logit of -infinity has probability 0 and is never listed: where fewer than
+ * top_k remain, the list ends in id -1, logprob -infinity. tokens[r] < 0 names
+ * no token: logprob 0 (a sum over a padded batch skips it); tokens[r] >= vocab
+ * gives NaN. A row of -infinity alone has entropy 0 and logprob -infinity. A
+ * row with a NaN or +infinity has no distribution: logprob, entropy and
+ * top_logprobs are NaN, ids -1. Needs no workspace. */
+#define TL_TOP_K_MAX 32
+TL_API tl_status tl_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, const int32_t* tokens,
+                                   int32_t rows, int32_t vocab, int32_t top_k, float* logprob, float* entropy,
+                                   int32_t* top_ids, float* top_logprobs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

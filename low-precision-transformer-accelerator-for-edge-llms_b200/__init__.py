@@ -9,7 +9,7 @@ any module name. The compute lives in ``libtl_b200.so``; ``shim`` is its
 ctypes binding and mirrors the reference's Python operator API.
 """
 
-from . import analysis, replicas, shim  # noqa: F401
+from . import analysis, replicas, serving, shim  # noqa: F401
 from .shim import (  # noqa: F401
     Engine, Linear, Layer, Model, TLError, check_model, checkpoint_config, forward_mixed, from_tinyllama_weights,
     layer_debug, load_checkpoint_npz, load_library, mixed_precision_decoder_layer, quantize_int8, quantize_weight,
@@ -17,3 +17,4 @@ from .shim import (  # noqa: F401
     contract_rope, residual_add_i32,
 )
 from .analysis import diff_stats, dump_debug, flatten_named_arrays, run_analysis  # noqa: F401
+from .serving import PagedKVCache, TokenLogprobs, token_logprobs  # noqa: F401

@@ -1,0 +1,87 @@
+// serving.cuh -- element types and addressing shared by the paged-cache and
+// log-probability operators (paged.cu, paged_attn.cu, logprobs.cu).
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "../../include/tl_api.h"
+#include "common.cuh"
+
+namespace tl {
+
+inline tl_status cuda_status(cudaError_t e) { return e == cudaSuccess ? TL_OK : TL_ERR_CUDA; }
+inline bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+inline int dtype_bytes(int32_t dt) { return dt == TL_F32 ? 4 : dt == TL_I8 ? 1 : 2; }
+inline bool is_float_dtype(int32_t dt) { return dt == TL_F32 || dt == TL_BF16 || dt == TL_F16; }
+
+template <typename T>
+TL_DEV float to_f32(T x);
+template <>
+TL_DEV float to_f32<float>(float x) { return x; }
+template <>
+TL_DEV float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+TL_DEV float to_f32<__half>(__half x) { return __half2float(x); }
+
+template <typename T>
+TL_DEV T from_f32(float x);
+template <>
+TL_DEV float from_f32<float>(float x) { return x; }
+template <>
+TL_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+TL_DEV __half from_f32<__half>(float x) { return __float2half_rn(x); }
+
+// Division of a position by the page size, which is any positive number: for
+// n < 2^31 and 1 <= d < 2^31 with s = ceil(log2 d), m = floor(2^(31+s) / d) + 1
+// fits 33 bits at most 2^32 and floor(n m / 2^(31+s)) = floor(n / d) (Granlund
+// and Montgomery, "Division by invariant integers using multiplication").
+struct PageDiv {
+  uint32_t d;
+  uint32_t shift;
+  uint64_t mul;
+};
+inline PageDiv page_div(int32_t d) {
+  PageDiv r;
+  r.d = static_cast<uint32_t>(d);
+  uint32_t s = 0;
+  while ((1ull << s) < r.d) ++s;
+  r.shift = 31 + s;
+  r.mul = (1ull << r.shift) / r.d + 1;
+  return r;
+}
+TL_DEV uint32_t div_page(uint32_t n, const PageDiv& p) {
+  return static_cast<uint32_t>((static_cast<uint64_t>(n) * p.mul) >> p.shift);
+}
+
+// The pool and the table as the kernels see them.
+struct PagedView {
+  void* k;
+  void* v;
+  float* ks;
+  float* vs;
+  int32_t pages, hkv, ps;
+  PageDiv div;
+  const int32_t* table;
+  int32_t n_seqs, max_pages;
+  int64_t table_stride;
+};
+
+// Row index (in rows of head_dim elements) of kv head 0 of position p of
+// sequence s, or -1 where none exists; head h is h * ps rows further.
+TL_DEV int64_t paged_row(const PagedView& c, int s, int p) {
+  if (s < 0 || s >= c.n_seqs || p < 0) return -1;
+  const uint32_t pg = div_page(static_cast<uint32_t>(p), c.div);
+  if (pg >= static_cast<uint32_t>(c.max_pages)) return -1;
+  const int page = c.table[static_cast<int64_t>(s) * c.table_stride + pg];
+  if (page < 0 || page >= c.pages) return -1;
+  return static_cast<int64_t>(page) * c.hkv * c.ps + (static_cast<uint32_t>(p) - pg * c.div.d);
+}
+
+// Checks shared by the paged entry points; fills the view.
+tl_status paged_view(const tl_paged_kv* cache, const int32_t* table, int32_t n_seqs, int32_t max_pages,
+                     int64_t table_stride, PagedView* out);
+
+}  // namespace tl

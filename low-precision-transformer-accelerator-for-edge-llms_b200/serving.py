@@ -1,0 +1,337 @@
+"""Paged KV cache and token log probabilities for callers that drive their own
+batch (include/tl_api.h, the paged cache section).
+
+Unlike the operators of :mod:`shim`, which mirror the reference's host
+functions, these take and return CUDA tensors: a server's cache, activations
+and logits stay on the device. Every call checks its arguments, enqueues one
+kernel on the current stream of the tensors' device and returns without
+synchronising; shapes, types, strides and devices that the library does not
+take raise ``ValueError``, errors of the library :class:`shim.TLError`. There
+is no CPU path.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple
+
+from .shim import check, load_library
+
+F32, BF16, F16, I8 = 0, 1, 2, 3  # tl_dtype
+TOP_K_MAX = 32
+HEAD_DIMS = (64, 128)
+
+_FLOAT_CODES: dict = {}
+_POOL_CODES: dict = {}
+
+
+class PagedView(C.Structure):
+    """tl_paged_kv"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("dtype", C.c_int32), ("num_pages", C.c_int32), ("kv_heads", C.c_int32), ("page_size", C.c_int32),
+                ("head_dim", C.c_int32)]
+
+
+def _torch():
+    import torch
+    if not _FLOAT_CODES:
+        _FLOAT_CODES.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+        _POOL_CODES.update({torch.int8: I8, torch.bfloat16: BF16, torch.float16: F16})
+    return torch
+
+
+def _bad(name, t, want):
+    got = f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}" if hasattr(t, "dtype") else type(t).__name__
+    return ValueError(f"{name} must be {want}, got {got}")
+
+
+def _index(name, t, n, dev):
+    """int32 vector of n entries on the device -> its address."""
+    torch = _torch()
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.shape == (n,) and t.device == dev
+            and (n < 2 or t.stride(0) == 1)):
+        raise _bad(name, t, f"a contiguous int32 [{n}] tensor on {dev}")
+    return t.data_ptr()
+
+
+def _rows(name, t, n, heads, d, dtype, dev):
+    """[n, heads, d] activations with contiguous head rows, 16-byte aligned -> (address, row stride)."""
+    torch = _torch()
+    if isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == (n, heads, d) and t.device == dev:
+        s0, s1, s2 = t.stride()
+        p = t.data_ptr()
+        if n < 2:
+            s0 = heads * d
+        if s2 == 1 and (s1 == d or heads == 1) and s0 >= heads * d and not (p | s0 * t.element_size()) & 15:
+            return p, s0
+    raise _bad(name, t, f"a {dtype} [{n}, {heads}, {d}] tensor on {dev}, head rows contiguous, tokens a multiple of "
+                        "16 bytes apart, 16-byte aligned")
+
+
+def _out(name, t, shape, dtype, dev):
+    """``t`` checked as a contiguous output, or a new tensor."""
+    torch = _torch()
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    if not (isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.device == dev
+            and t.is_contiguous() and not t.data_ptr() & 15):
+        raise _bad(name, t, f"a contiguous {dtype} {list(shape)} tensor on {dev}, 16-byte aligned")
+    return t
+
+
+class PagedKVCache:
+    """One layer's pool of KV pages (tl_paged_kv).
+
+    ``k`` and ``v`` are ``[num_pages, kv_heads, page_size, head_dim]`` tensors of
+    int8, bfloat16 or float16; an int8 pool has float32 ``k_scale`` and
+    ``v_scale`` ``[num_pages, kv_heads, page_size]``, one scale per stored row.
+    ``head_dim`` is 64 or 128, ``page_size`` any positive number.
+
+    The caller owns the page allocation: position ``p`` of sequence ``s`` is row
+    ``p % page_size`` of page ``block_table[s, p // page_size]`` (int32 on the
+    device). Entries that name no sequence, position or page are skipped (see
+    each call), so a batch of fixed size is padded with ``seq = -1``. Calls on
+    one cache are serialized by the caller, as on an engine: on one stream, or
+    ordered by events. No call synchronises or allocates beyond its outputs
+    (taken from torch's allocator), so with preallocated outputs calls can be
+    captured in a CUDA graph.
+    """
+
+    def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=None, device="cuda"):
+        """Allocates the pool, zeroed; ``dtype`` is torch.int8 (default), bfloat16 or float16."""
+        torch = _torch()
+        dtype = torch.int8 if dtype is None else dtype
+        if dtype not in _POOL_CODES:
+            raise ValueError(f"dtype must be one of {[str(x) for x in _POOL_CODES]}, got {dtype}")
+        if min(num_pages, page_size, kv_heads) < 1 or head_dim not in HEAD_DIMS:
+            raise ValueError(f"num_pages, page_size and kv_heads must be positive and head_dim one of {HEAD_DIMS}")
+        if not torch.cuda.is_available():
+            raise RuntimeError("no CUDA device visible: the paged cache runs only on the GPU")
+        shape = (num_pages, kv_heads, page_size, head_dim)
+        k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+        ks, vs = ((torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
+                  if dtype == torch.int8 else (None, None))
+        self._bind(k, v, ks, vs)
+
+    @classmethod
+    def from_tensors(cls, k, v, k_scale=None, v_scale=None) -> "PagedKVCache":
+        """A cache over tensors the caller owns (one layer's slice of a larger pool, for instance)."""
+        self = cls.__new__(cls)
+        self._bind(k, v, k_scale, v_scale)
+        return self
+
+    def _bind(self, k, v, k_scale, v_scale):
+        torch = _torch()
+        for name, t in (("k", k), ("v", v)):
+            if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 4 and t.dtype in _POOL_CODES
+                    and t.numel() and t.is_contiguous() and not t.data_ptr() & 15):
+                raise _bad(name, t, "a contiguous, 16-byte aligned CUDA tensor [num_pages, kv_heads, page_size, "
+                                    "head_dim] of int8, bfloat16 or float16")
+        if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise ValueError("k and v must agree in shape, type and device")
+        if k.shape[3] not in HEAD_DIMS:
+            raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {k.shape[3]}")
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if k.dtype != torch.int8:
+                if t is not None:
+                    raise ValueError(f"{name} is for int8 pools only")
+            elif not (isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.shape == k.shape[:3]
+                      and t.device == k.device and t.is_contiguous()):
+                raise _bad(name, t, f"a contiguous float32 {list(k.shape[:3])} tensor on {k.device}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        self.dtype, self.device = k.dtype, k.device
+        self._lib = load_library()
+        ptr = [t.data_ptr() if t is not None else None for t in (k, v, k_scale, v_scale)]
+        self._view = PagedView(*ptr, _POOL_CODES[k.dtype], *k.shape)
+        self._ref = C.byref(self._view)
+        self._scale = self.head_dim ** -0.5
+        self._work = None
+        self._work_bytes = 0
+
+    # ---------------------------------------------------------------- calls
+    def _call(self, name, *args):
+        torch = _torch()
+        if torch.cuda.current_device() == self.device.index:
+            code = getattr(self._lib, name)(*args, torch.cuda.current_stream().cuda_stream)
+        else:
+            with torch.cuda.device(self.device):
+                code = getattr(self._lib, name)(*args, torch.cuda.current_stream().cuda_stream)
+        if code:
+            check(code, name)
+
+    def _table(self, t):
+        torch = _torch()
+        if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == 2 and t.device == self.device
+                and t.shape[0] and t.shape[1] and (t.shape[1] == 1 or t.stride(1) == 1)):
+            raise _bad("block_table", t, f"an int32 [n_seqs, max_pages] tensor on {self.device} with contiguous rows")
+        n, m = t.shape
+        stride = t.stride(0) if n > 1 else m
+        if stride < m:
+            raise _bad("block_table", t, "a table whose rows do not overlap")
+        return t.data_ptr(), n, m, stride
+
+    def append(self, k, v, block_table, seq, pos, cos=None, sin=None, q=None, q_out=None):
+        """Stores key and value rows ``k``, ``v`` ``[tokens, kv_heads, head_dim]`` at
+        ``(seq[t], pos[t])``, the keys rotated by their position on the way
+        (tl_paged_append).
+
+        ``cos`` and ``sin`` are :func:`shim.rope_tables`' float32 ``[max_positions,
+        head_dim]`` on the device. ``q`` ``[tokens, heads, head_dim]`` is rotated too
+        and returned (in ``q_out`` when given; ``q_out is q`` rotates a contiguous
+        ``q`` in place); without ``q`` the result is None. Without ``cos`` and
+        ``sin`` the keys are stored as they are. ``k``, ``v`` and ``q`` are float32,
+        bfloat16 or float16 and may be columns of one fused projection. Tokens
+        that name no row store nothing; a position beyond the angles stores
+        nothing and gives a zero query row.
+        """
+        torch = _torch()
+        if not isinstance(k, torch.Tensor) or k.dim() != 3 or k.dtype not in _FLOAT_CODES:
+            raise _bad("k", k, "a float32, bfloat16 or float16 [tokens, kv_heads, head_dim] tensor")
+        n, dt, dev, d = k.shape[0], k.dtype, self.device, self.head_dim
+        kp, ks = _rows("k", k, n, self.kv_heads, d, dt, dev)
+        vp, vs = _rows("v", v, n, self.kv_heads, d, dt, dev)
+        tab = self._table(block_table)
+        sp, pp = _index("seq", seq, n, dev), _index("pos", pos, n, dev)
+        if (cos is None) != (sin is None):
+            raise ValueError("cos and sin go together")
+        cp = np_ = n_ang = None
+        if cos is not None:
+            for name, t in (("cos", cos), ("sin", sin)):
+                if not (isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.dim() == 2 and t.shape[0]
+                        and t.shape[1] == d and t.shape == cos.shape and t.device == dev and t.is_contiguous()
+                        and not t.data_ptr() & 15):
+                    raise _bad(name, t, f"a contiguous float32 [max_positions, {d}] tensor on {dev}")
+            cp, np_, n_ang = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+        qp, qs, heads, op = None, 0, 0, None
+        if q is not None:
+            if cos is None:
+                raise ValueError("q needs cos and sin")
+            if not isinstance(q, torch.Tensor) or q.dim() != 3 or not q.shape[1]:
+                raise _bad("q", q, "a [tokens, heads, head_dim] tensor")
+            heads = q.shape[1]
+            qp, qs = _rows("q", q, n, heads, d, dt, dev)
+            q_out = _out("q_out", q_out, (n, heads, d), dt, dev)
+            op = q_out.data_ptr()
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        if n:
+            self._call("tl_paged_append", self._ref, qp, kp, vp, _FLOAT_CODES[dt], qs, ks, vs, sp, pp, *tab, cp, np_,
+                       n_ang or 0, n, heads, op)
+        return q_out
+
+    def read(self, block_table, seq, pos, dtype=None, k_out=None, v_out=None):
+        """Rows ``(seq[t], pos[t])`` as ``(k, v)``, each ``[tokens, kv_heads, head_dim]`` of
+        ``dtype`` (float32 by default; tl_paged_read). Keys are as stored, rotated.
+        Tokens that name no row give zeros."""
+        torch = _torch()
+        dtype = torch.float32 if dtype is None else dtype
+        if dtype not in _FLOAT_CODES:
+            raise ValueError(f"dtype must be one of {[str(x) for x in _FLOAT_CODES]}, got {dtype}")
+        if not isinstance(seq, torch.Tensor) or seq.dim() != 1:
+            raise _bad("seq", seq, "an int32 vector")
+        n, dev = seq.shape[0], self.device
+        tab = self._table(block_table)
+        sp, pp = _index("seq", seq, n, dev), _index("pos", pos, n, dev)
+        shape = (n, self.kv_heads, self.head_dim)
+        k, v = _out("k_out", k_out, shape, dtype, dev), _out("v_out", v_out, shape, dtype, dev)
+        if n:
+            self._call("tl_paged_read", self._ref, sp, pp, *tab, n, k.data_ptr(), v.data_ptr(), _FLOAT_CODES[dtype])
+        return k, v
+
+    def attend(self, q, block_table, lengths, seq=None, sm_scale=None, out=None, return_lse=False, lse=None):
+        """Attention of one new token of each row's sequence over its first
+        ``lengths[r]`` positions (tl_paged_attn_decode).
+
+        ``q`` ``[rows, heads, head_dim]`` is already rotated (:meth:`append` returns
+        it), float32, bfloat16 or float16 whatever the pool's type; ``heads`` is any
+        multiple of ``kv_heads``. Row ``r`` reads sequence ``seq[r]`` (default
+        ``r``). ``sm_scale`` defaults to ``head_dim ** -0.5``. Returns ``out`` of
+        ``q``'s shape and type, with ``return_lse`` also the float32 log-sum-exp
+        ``[rows, heads]`` of the scores. A row without positions gives zeros and
+        -inf.
+        """
+        torch = _torch()
+        if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _FLOAT_CODES:
+            raise _bad("q", q, "a float32, bfloat16 or float16 [rows, heads, head_dim] tensor")
+        n, heads, d = q.shape
+        dt, dev = q.dtype, self.device
+        if d != self.head_dim or not heads or heads % self.kv_heads:
+            raise ValueError(f"q has {heads} heads of {d}: the pool has {self.kv_heads} heads of {self.head_dim}, and "
+                             "q's must be a multiple")
+        qp, qs = _rows("q", q, n, heads, d, dt, dev)
+        tab = self._table(block_table)
+        lp = _index("lengths", lengths, n, dev)
+        if seq is not None:
+            sp = _index("seq", seq, n, dev)
+        elif n > tab[1]:
+            raise ValueError(f"{n} rows but the table has {tab[1]} sequences: pass seq")
+        else:
+            sp = None
+        out = _out("out", out, (n, heads, d), dt, dev)
+        if return_lse or lse is not None:
+            lse = _out("lse", lse, (n, heads), torch.float32, dev)
+        if n:
+            work = self._workspace(heads)
+            self._call("tl_paged_attn_decode", self._ref, qp, _FLOAT_CODES[dt], qs, sp, lp, *tab, n, heads,
+                       self._scale if sm_scale is None else float(sm_scale), out.data_ptr(),
+                       lse.data_ptr() if lse is not None else None, work, self._work_bytes)
+        return (out, lse) if return_lse else out
+
+    def _workspace(self, heads):
+        """The cache's own scratch, allocated at the first call with so many heads
+        (make that call before capturing a graph) and kept: its size does not
+        depend on rows or lengths."""
+        if self._work is None or self._work[1] < heads:
+            torch = _torch()
+            need = self._lib.tl_paged_attn_workspace_bytes(heads, self.kv_heads, self.head_dim)
+            kept = self._work  # a larger one may follow while calls that use this one are in flight
+            if need > self._work_bytes:
+                t = torch.zeros(need, dtype=torch.uint8, device=self.device)
+                self._work, self._work_bytes = (t, heads, kept), need
+            else:
+                self._work = (kept[0], heads, kept[2])
+        return self._work[0].data_ptr()
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: object       # float32 [rows], None without tokens
+    entropy: object       # float32 [rows]
+    top_ids: object       # int32 [rows, top_k]
+    top_logprobs: object  # float32 [rows, top_k]
+
+
+def token_logprobs(logits, tokens=None, top_k: int = 0) -> TokenLogprobs:
+    """Log probabilities of ``tokens`` (int32 ``[rows]``), the entropy and the
+    ``top_k`` (at most 32) most likely tokens of each row of ``logits``
+    ``[rows, vocab]`` (float32, bfloat16 or float16; rows may be strided), in one
+    pass over them (tl_token_logprobs). Equal logits are listed by the lowest
+    id. Logits of -inf have probability 0 and are never listed (id -1, -inf).
+    A negative token gives 0, one beyond the vocabulary NaN; a row with a NaN or
+    +inf gives NaN everywhere."""
+    torch = _torch()
+    if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dim() == 2 and logits.dtype in _FLOAT_CODES
+            and logits.shape[1] and (logits.shape[1] == 1 or logits.stride(1) == 1)):
+        raise _bad("logits", logits, "a CUDA tensor [rows, vocab] of float32, bfloat16 or float16 with contiguous rows")
+    n, vocab = logits.shape
+    dev = logits.device
+    stride = logits.stride(0) if n > 1 else vocab
+    if stride < vocab:
+        raise _bad("logits", logits, "rows that do not overlap")
+    if not 0 <= top_k <= TOP_K_MAX:
+        raise ValueError(f"top_k must be in 0..{TOP_K_MAX}, got {top_k}")
+    tp = _index("tokens", tokens, n, dev) if tokens is not None else None
+    f32 = torch.float32
+    lp = torch.empty(n, dtype=f32, device=dev) if tokens is not None else None
+    ent = torch.empty(n, dtype=f32, device=dev)
+    ids = torch.empty((n, top_k), dtype=torch.int32, device=dev)
+    top = torch.empty((n, top_k), dtype=f32, device=dev)
+    if n:
+        with torch.cuda.device(dev):
+            code = load_library().tl_token_logprobs(
+                logits.data_ptr(), _FLOAT_CODES[logits.dtype], stride, tp, n, vocab, top_k,
+                lp.data_ptr() if lp is not None else None, ent.data_ptr(), ids.data_ptr() if top_k else None,
+                top.data_ptr() if top_k else None, torch.cuda.current_stream().cuda_stream)
+        if code:
+            check(code, "tl_token_logprobs")
+    return TokenLogprobs(lp, ent, ids, top)
