@@ -13,8 +13,11 @@ tl_status paged_view(const tl_paged_kv* c, const int32_t* table, int32_t n_seqs,
   if (c->num_pages <= 0 || c->kv_heads <= 0 || c->page_size <= 0) return TL_ERR_INVALID_ARGUMENT;
   if (n_seqs <= 0 || max_pages <= 0 || table_stride < max_pages) return TL_ERR_INVALID_ARGUMENT;
   if (!aligned_to(c->k, 16) || !aligned_to(c->v, 16) || !aligned_to(table, 4)) return TL_ERR_INVALID_ARGUMENT;
-  // positions are 32-bit
-  if (static_cast<int64_t>(max_pages) * c->page_size > INT32_MAX) return TL_ERR_OUT_OF_RANGE;
+  // positions and row indexes are 31-bit, with room to round a length up
+  constexpr int64_t kMost = INT32_MAX - 4096;
+  if (static_cast<int64_t>(max_pages) * c->page_size > kMost ||
+      static_cast<int64_t>(c->num_pages) * c->kv_heads > kMost / c->page_size)
+    return TL_ERR_OUT_OF_RANGE;
   out->k = c->k;
   out->v = c->v;
   out->ks = c->k_scale;
