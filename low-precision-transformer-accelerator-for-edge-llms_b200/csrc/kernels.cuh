@@ -96,6 +96,9 @@ struct TcPlan {
 cudaError_t tc_make_plan(TcPlan* p, const int8_t* w_nk, int N, const int8_t* x, int M, int K, int num_sms, int epi);
 // Tensor map of a [rows][64] fp16 matrix in SW128 boxes of box_rows rows.
 cudaError_t tc_encode_f16_rows64(CUtensorMap* tm, const void* base, long long rows, int box_rows);
+// Tensor map of [rows][row_bytes] bytes (64 or a multiple of 128) in boxes of box_rows rows of 64 bytes (SW64) or
+// 128 bytes (SW128).
+cudaError_t tc_encode_rows_bytes(CUtensorMap* tm, const void* base, long long rows, int row_bytes, int box_rows);
 cudaError_t launch_gemm_tc(const TcPlan& p, const TcArgs& a, cudaStream_t s, bool pdl);
 cudaError_t prepare_tc();
 int tc_max_stages(int bn, int ks = 1);
@@ -184,6 +187,8 @@ int attn_splits(int M, int Hkv, int P);
 size_t attn_part_floats(int M, int Hkv, int P);
 cudaError_t attn_prepare();
 cudaError_t attn_read_error(unsigned int* code);
+// The same for the paged attention kernel (paged_attn.cu).
+cudaError_t paged_attn_read_error(unsigned int* code);
 
 // ---- prefill helpers (rows of n_seq sequences of seq_len tokens each)
 cudaError_t launch_embed(const float* table, const int* ids, float* x, int rows, int D,

@@ -38,6 +38,7 @@ tl_status tl_device_error(void) {
   unsigned int code = 0;
   if (cudaDeviceSynchronize() != cudaSuccess) return TL_ERR_CUDA;
   if (tc_read_error(&code) != cudaSuccess) return TL_ERR_CUDA;
+  if (code == 0 && paged_attn_read_error(&code) != cudaSuccess) return TL_ERR_CUDA;
   return code ? TL_ERR_TIMEOUT : TL_OK;
 }
 

@@ -11,9 +11,9 @@
 // group's query heads only (a few operations a byte), so the bound is the
 // rate of reading the pool. Everything else has to hide behind the loads:
 //  * work is split evenly over the CTAs whatever the lengths are (below);
-//  * each warp owns a ring of tiles filled by cp.async two tiles ahead, and
-//    each thread's copies are exactly the 16-byte pieces that its own MMA
-//    fragments need: no bank conflicts, no transposes, no barriers;
+//  * each warp owns a ring of tiles that TMA fills ahead of it (boxes of rows
+//    of one page, 128-byte swizzle), so that no instruction of the warp moves
+//    data and ldmatrix reads the operands without bank conflicts;
 //  * both products run on mma.sync m16n8k16. A group has few rows, so a
 //    128-row tcgen05 tile would be mostly padding and its result would have
 //    to come back through tensor memory; the 16-row tile is small enough to
@@ -30,12 +30,33 @@
 // Accumulators, maxima and sums are float32.
 #include <algorithm>
 
+#include <numeric>
+
 #include "kernels.cuh"
 #include "serving.cuh"
+#include "tc_common.cuh"
 
 namespace tl {
 namespace {
 
+#ifndef VAR_S64
+#define VAR_S64 4
+#endif
+#ifndef VAR_S128
+#define VAR_S128 3
+#endif
+#ifndef VAR_S256
+#define VAR_S256 3
+#endif
+#ifndef VAR_C64
+#define VAR_C64 3
+#endif
+#ifndef VAR_C128
+#define VAR_C128 2
+#endif
+#ifndef VAR_C256
+#define VAR_C256 2
+#endif
 constexpr int kWarps = 4;         // warps of a CTA, each on its own tiles
 constexpr int kMaxCtas = 640;     // grid bound (148 SMs x 4 CTAs), sizes the workspace
 constexpr float kLog2e = 1.4426950408889634f;
@@ -47,6 +68,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kHeadroom = 8.0f;
 constexpr float kLazy = 6.0f;
 
+// Set when a wait on a tile ran out (tl_device_error reads and clears it).
+__device__ unsigned int g_paged_error = 0;
+
 struct AttendArgs {
   PagedView c;
   const void* q;
@@ -57,19 +81,13 @@ struct AttendArgs {
   float scale;
   void* out;
   float* lse;
+  int32_t box;            // rows of a TMA box: the largest that divides a page and a tile
   unsigned int* tickets;  // [kMaxCtas], zero between calls
   float* records;         // [kMaxCtas][2][kHeads][D + 2]
 };
 
-TL_DEV void cp_async16(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(src)), "r"(live ? 16 : 0)
-               : "memory");
-}
-TL_DEV void cp_async8(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)),
-               "r"(live ? 8 : 0)
-               : "memory");
+TL_DEV void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)) : "memory");
 }
 TL_DEV void cp_async4(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)),
@@ -80,14 +98,19 @@ TL_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memor
 template <int N>
 TL_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-TL_DEV uint4 lds16(uint32_t a) {
+// Four 8x8 matrices of 16-bit elements, lane l's address naming row l % 8 of
+// matrix l / 8; TRANS transposes each.
+template <bool TRANS>
+TL_DEV uint4 ldmatrix4(uint32_t addr) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-TL_DEV uint2 lds8(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr));
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr));
   return v;
 }
 TL_DEV float exp2_approx(float x) {
@@ -99,13 +122,11 @@ TL_DEV float exp2_approx(float x) {
 template <bool BF>
 TL_DEV void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   if constexpr (BF)
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -142,23 +163,24 @@ struct Shape {
   static constexpr int HEADS = 8 * MT;                  // query heads of a CTA
   static constexpr int RB = D * (I8 ? 1 : 2);           // bytes of a stored row
   static constexpr int KT = RB == 256 ? 16 : 32;        // positions of a warp's tile
-  static constexpr int KSEG = RB / 64;                  // 16-byte key pieces of a thread and position
+  static constexpr int SUB = RB < 128 ? RB : 128;       // bytes of a row in one box
+  static constexpr int NSUB = RB / SUB;
   static constexpr int KS = D / 16;                     // MMA steps over head_dim
-  static constexpr int VB = RB == 64 ? 8 : 16;          // bytes of a value piece
-  static constexpr int CH = VB / (I8 ? 1 : 2);          // its elements
-  static constexpr int VSEG = RB / (8 * VB);            // value pieces of a thread and position
-  static constexpr int KBYTES = KT / 8 * KSEG * 512;
-  static constexpr int VBYTES = KT / 4 * VSEG * 32 * VB;
-  static constexpr int SCALES = KBYTES + VBYTES;        // offset of the tile's scales, then its mask
-  static constexpr int MASK = SCALES + (I8 ? 2 * KT * 4 : 0);
-  static constexpr int PITCH = D + 4;                   // floats between heads of a partial result
-  static constexpr int MERGE = (HEADS * PITCH + 2 * HEADS) * 4;
-  static constexpr int STAGE = ((MASK + 16 > MERGE ? MASK + 16 : MERGE) + 127) / 128 * 128;
-  static constexpr int STAGES = RB == 64 ? 4 : 3;
-  static constexpr int SMEM = kWarps * STAGES * STAGE;
+  static constexpr int HALF = KT * RB;                  // bytes of a tile's keys, of its values
+  static constexpr int MERGE = HEADS * D * 4;           // a warp's partial result, in a tile it has read
+  static constexpr int STAGE = 2 * HALF;
+  static_assert(MERGE <= STAGE && STAGE % 1024 == 0 && (KT * SUB) % 1024 == 0, "swizzled boxes, partial results");
+  static constexpr int STAGES = RB == 64 ? VAR_S64 : RB == 128 ? VAR_S128 : VAR_S256;
+  // shared memory: rings, then scales (int8), tile masks, partial m and l, barriers
+  static constexpr int RING = kWarps * STAGES * STAGE;
+  static constexpr int SCALES = RING;
+  static constexpr int MASKS = SCALES + (I8 ? kWarps * STAGES * 2 * KT * 4 : 0);
+  static constexpr int STATS = MASKS + kWarps * STAGES * 4;
+  static constexpr int BARS = (STATS + kWarps * 2 * HEADS * 4 + 7) / 8 * 8;
+  static constexpr int SMEM = BARS + kWarps * STAGES * 8 + 1024;  // the base is rounded up to 1024
   static constexpr int UNIT = kWarps * KT;              // positions of one CTA round
   static constexpr int RECORD = HEADS * (D + 2);        // floats of a partial result in the workspace
-  static constexpr int CTAS = MT == 2 ? 2 : RB == 64 ? 3 : 2;  // CTAs an SM holds
+  static constexpr int CTAS = MT == 2 ? 2 : RB == 64 ? VAR_C64 : RB == 128 ? VAR_C128 : VAR_C256;  // CTAs an SM holds
 };
 
 // Length of row r in positions, 0 for rows that name no sequence.
@@ -209,10 +231,11 @@ TL_DEV void store_out(void* out, int dt, int64_t i, float4 v) {
         make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
   }
 }
-TL_DEV float load_act(const void* p, int dt, int64_t i) {
-  return dt == TL_F32    ? static_cast<const float*>(p)[i]
-         : dt == TL_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i])
-                         : __half2float(static_cast<const __half*>(p)[i]);
+TL_DEV float2 load_act2(const void* p, int dt, int64_t i) {
+  if (dt == TL_F32) return *reinterpret_cast<const float2*>(static_cast<const float*>(p) + i);
+  if (dt == TL_BF16)
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(static_cast<const __nv_bfloat16*>(p) + i));
+  return __half22float2(*reinterpret_cast<const __half2*>(static_cast<const __half*>(p) + i));
 }
 
 // Rows without positions are on nobody's line: zeros and -infinity.
@@ -237,9 +260,12 @@ TL_DEV void zero_empty_rows(const AttendArgs& a) {
 // counts them) joins them in CTA order, so the result does not depend on the
 // order of arrival.
 template <typename S>
-__global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, S::CTAS)
+    attend_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v) {
   constexpr int D = S::D, MT = S::MT, KT = S::KT, UNIT = S::UNIT;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ int sh_units[kWarps];
   __shared__ int sh_first[2];  // first row of the stretch, units before it
   __shared__ int sh_last;
@@ -299,7 +325,17 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
   Place fill = use;
 
   // ---- the warp's ring
-  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * S::STAGES * S::STAGE;
+  unsigned char* ring = smem + warp * S::STAGES * S::STAGE;
+  const uint32_t ring32 = smem_u32(ring);
+  float* scales = reinterpret_cast<float*>(smem + S::SCALES) + warp * S::STAGES * 2 * KT;
+  unsigned* masks = reinterpret_cast<unsigned*>(smem + S::MASKS) + warp * S::STAGES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BARS) + warp * S::STAGES;
+  if (lane == 0) {
+    for (int i = 0; i < S::STAGES; ++i) mbar_init(bars + i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+  bool late = false;  // a wait has run out: the results are void, the host learns of it
   // Row index of position `lane` of the tile at `p` (lanes < KT), -1: none.
   auto lookup = [&](const Place& p) -> int {
     const int pos = (p.rd * kWarps + warp) * KT + lane;
@@ -309,38 +345,43 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
     if (page < 0 || page >= a.c.pages) return -1;
     return (page * a.c.hkv + p.it / a.blocks) * a.c.ps + (pos - static_cast<int>(pg * a.c.div.d));
   };
+  // Boxes start at multiples of a.box positions and lie within one page, so a
+  // box exists if its first position does (rows past the length stay unused).
   auto copy_tile = [&](int stage, int row) {
-    const uint32_t base = ring + stage * S::STAGE;
+    // TMA writes whole 128 bytes: single rows of 64 bytes (odd page sizes) are copied by the lanes
+    const bool tma = S::SUB == 128 || a.box > 1;
     const unsigned live = __ballot_sync(0xffffffffu, row >= 0);
-    if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + S::MASK), "r"(live) : "memory");
-    if (live == 0) return;  // nothing of the tile will be read
-    const char* kp = static_cast<const char*>(a.c.k) + t * 16;
-    const char* vp = static_cast<const char*>(a.c.v) + g * S::VB;
-#pragma unroll
-    for (int j = 0; j < KT / 8; ++j) {
-      const int r = __shfl_sync(0xffffffffu, row, 8 * j + g);
-      const char* src = kp + static_cast<int64_t>(max(r, 0)) * S::RB;
-#pragma unroll
-      for (int s = 0; s < S::KSEG; ++s)
-        cp_async16(base + (j * S::KSEG + s) * 512 + lane * 16, src + s * 64, r >= 0);
+    const bool head = tma && row >= 0 && lane % a.box == 0;
+    const unsigned boxes = __ballot_sync(0xffffffffu, head);
+    if (lane == 0) {
+      masks[stage] = live;
+      mbar_arrive_expect_tx(bars + stage, __popc(boxes) * a.box * S::RB * 2);
     }
+    unsigned char* dst = ring + stage * S::STAGE + lane * S::SUB;
+    if (head) {
 #pragma unroll
-    for (int j = 0; j < KT / 4; ++j) {
-      const int r = __shfl_sync(0xffffffffu, row, 16 * (j >> 2) + 8 * ((j >> 1) & 1) + 2 * t + (j & 1));
-      const char* src = vp + static_cast<int64_t>(max(r, 0)) * S::RB;
+      for (int s = 0; s < S::NSUB; ++s) {
+        tma_load_2d(dst + s * KT * S::SUB, &tm_k, s * S::SUB, row, bars + stage);
+        tma_load_2d(dst + S::HALF + s * KT * S::SUB, &tm_v, s * S::SUB, row, bars + stage);
+      }
+    }
+    if constexpr (S::SUB == 64) {
+      if (!tma && row >= 0) {
+        const char* kp = static_cast<const char*>(a.c.k) + static_cast<int64_t>(row) * 64;
+        const char* vp = static_cast<const char*>(a.c.v) + static_cast<int64_t>(row) * 64;
 #pragma unroll
-      for (int s = 0; s < S::VSEG; ++s) {
-        const uint32_t dst = base + S::KBYTES + (j * S::VSEG + s) * 32 * S::VB + lane * S::VB;
-        if constexpr (S::VB == 16)
-          cp_async16(dst, src + s * 128, r >= 0);
-        else
-          cp_async8(dst, src, r >= 0);
+        for (int p = 0; p < 4; ++p) {
+          const int at = (p ^ (lane >> 1 & 3)) * 16;
+          cp_async16(smem_u32(dst) + at, kp + p * 16);
+          cp_async16(smem_u32(dst) + S::HALF + at, vp + p * 16);
+        }
       }
     }
     if constexpr (S::I8) {
       if (lane < KT) {
-        cp_async4(base + S::SCALES + lane * 4, a.c.ks + max(row, 0), row >= 0);
-        cp_async4(base + S::SCALES + KT * 4 + lane * 4, a.c.vs + max(row, 0), row >= 0);
+        float* sc = scales + stage * 2 * KT + lane;
+        cp_async4(smem_u32(sc), a.c.ks + max(row, 0), row >= 0);
+        cp_async4(smem_u32(sc + KT), a.c.vs + max(row, 0), row >= 0);
       }
     }
   };
@@ -352,9 +393,16 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
       fill.next<UNIT>(a, items);
       ++filled;
     }
-    cp_async_commit();
+    if constexpr (S::I8) cp_async_commit();
   }
   int next_row = filled < n_units ? lookup(fill) : -1;
+
+  // Byte offsets of this lane's ldmatrix rows, swizzled: 16-byte piece c of row
+  // r of a box lies at piece c ^ (r % 8) of 128-byte rows, c ^ (r / 2 % 4) of
+  // 64-byte rows. Row offsets that are multiples of 8 leave the swizzle alone.
+  const int l8 = lane & 7, v_row = lane & 15;
+  const uint32_t k_lane = l8 * S::SUB + (((lane >> 3) ^ (S::SUB == 128 ? l8 : l8 >> 1)) << 4);
+  const uint32_t v_lane = v_row * S::SUB + (((lane >> 4) ^ (S::SUB == 128 ? l8 : l8 >> 1)) << 4);
 
   // ---- the running state of one item
   uint32_t qa[MT][S::KS][4];                       // query, high and low rows
@@ -365,7 +413,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
   float vu = 0.0f, vinv = 1.0f;  // int8: the power of two that value scales are divided by, its inverse
   bool fresh = true;
 
-  for (int i = 0, stage = 0; i < n_units; ++i, stage = stage + 1 == S::STAGES ? 0 : stage + 1) {
+  for (int i = 0, stage = 0, phase = 0; i < n_units; ++i) {
     if (fresh) {
       fresh = false;
       const int kvh = use.it / a.blocks, hb = use.it % a.blocks;
@@ -376,12 +424,14 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
         const int64_t base = use.r * a.ldq + static_cast<int64_t>(kvh * a.group + (live ? hg : 0)) * D;
         float x[D / 4];
         float top = 0.0f;
-        constexpr int RUN = S::I8 ? 16 : 8;  // consecutive elements of a thread
 #pragma unroll
-        for (int e = 0; e < D / 4; ++e) {
-          const int d = e / RUN * 4 * RUN + t * RUN + e % RUN;
-          x[e] = live ? load_act(a.q, a.q_dtype, base + d) : 0.0f;
-          top = fmaxf(top, fabsf(x[e]));
+        for (int e = 0; e < D / 4; e += 2) {
+          // the elements that the key fragments hold for this lane
+          const int d = e / 4 * 16 + (S::I8 ? t * 4 + e % 4 : t * 2 + e % 4 * 4);
+          const float2 y = live ? load_act2(a.q, a.q_dtype, base + d) : make_float2(0.0f, 0.0f);
+          x[e] = y.x;
+          x[e + 1] = y.y;
+          top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -415,7 +465,8 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
       vinv = 0.0f;
     }
 
-    cp_async_wait<S::STAGES - 2>();
+    if (late ? !mbar_try_wait(bars + stage, phase) : !mbar_wait_err(bars + stage, phase, 1u, &g_paged_error)) late = true;
+    if constexpr (S::I8) cp_async_wait<S::STAGES - 2>();
     __syncwarp();
     // refill the stage consumed one round ago
     if (filled < n_units) {
@@ -424,22 +475,38 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
       ++filled;
       next_row = filled < n_units ? lookup(fill) : -1;
     }
-    cp_async_commit();
+    if constexpr (S::I8) cp_async_commit();
 
-    const uint32_t base = ring + stage * S::STAGE;
-    unsigned live;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(live) : "r"(base + S::MASK));
+    const uint32_t kbase = ring32 + stage * S::STAGE, vbase = kbase + S::HALF;
+    const float* sc = scales + stage * 2 * KT;
+    const unsigned live = masks[stage];
+    if constexpr (!S::I8) {
+      // values of positions that do not exist must not meet a probability of zero as a NaN
+      constexpr unsigned full = KT == 32 ? 0xffffffffu : 0xffffu;
+      if (live != 0 && live != full) {
+        for (int r = 0; r < KT; ++r)
+          if (!(live >> r & 1) && lane < S::RB / 16)
+            *reinterpret_cast<uint4*>(ring + stage * S::STAGE + S::HALF + (lane / (S::SUB / 16) * KT + r) * S::SUB +
+                                      lane % (S::SUB / 16) * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();  // before TMA writes there again
+        __syncwarp();
+      }
+    }
     if (live) {
       // ---- scores: s[mt][j] of positions 8 j + 2 t, + 1 for head g
       float s[MT][KT / 8][2];
+      float c[KT / 8][MT][4];
 #pragma unroll
-      for (int j = 0; j < KT / 8; ++j) {
-        float c[MT][4];
+      for (int j = 0; j < KT / 8; ++j)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) c[mt][0] = c[mt][1] = c[mt][2] = c[mt][3] = 0.0f;
+        for (int mt = 0; mt < MT; ++mt) c[j][mt][0] = c[j][mt][1] = c[j][mt][2] = c[j][mt][3] = 0.0f;
+      // 64 bytes of a key row at a time: lane l reads row l % 8, piece l / 8
 #pragma unroll
-        for (int sg = 0; sg < S::KSEG; ++sg) {
-          const uint4 w = lds16(base + (j * S::KSEG + sg) * 512 + lane * 16);
+      for (int q = 0; q < S::RB / 64; ++q)
+#pragma unroll
+        for (int j = 0; j < KT / 8; ++j) {
+          const uint4 w = ldmatrix4<false>(kbase + (q * 64 / S::SUB * KT + 8 * j) * S::SUB +
+                                           (q * 64 % S::SUB ^ k_lane));
           const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int k = 0; k < (S::I8 ? 4 : 2); ++k) {
@@ -452,26 +519,27 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
               b0 = ww[2 * k];
               b1 = ww[2 * k + 1];
             }
-            const int ks = sg * (S::I8 ? 4 : 2) + k;
+            const int ks = q * (S::I8 ? 4 : 2) + k;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              mma16<S::BF>(c[mt], qa[mt][ks], b0, b1);
+              mma16<S::BF>(c[j][mt], qa[mt][ks], b0, b1);
               if constexpr (S::PARTS == 3) {
                 const uint32_t third[4] = {qc[mt][ks][0], 0u, qc[mt][ks][1], 0u};
-                mma16<S::BF>(c[mt], third, b0, b1);
+                mma16<S::BF>(c[j][mt], third, b0, b1);
               }
             }
           }
         }
+#pragma unroll
+      for (int j = 0; j < KT / 8; ++j) {
         float2 kscale = make_float2(1.0f, 1.0f);
         if constexpr (S::I8) {
-          const uint2 w = lds8(base + S::SCALES + (8 * j + 2 * t) * 4);
-          kscale = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+          kscale = *reinterpret_cast<const float2*>(sc + 8 * j + 2 * t);
         }
         const bool in0 = live >> (8 * j + 2 * t) & 1, in1 = live >> (8 * j + 2 * t + 1) & 1;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          float x = (c[mt][0] + c[mt][2]) * qscale[mt], y = (c[mt][1] + c[mt][3]) * qscale[mt];
+          float x = (c[j][mt][0] + c[j][mt][2]) * qscale[mt], y = (c[j][mt][1] + c[j][mt][3]) * qscale[mt];
           if constexpr (S::I8) {
             x *= kscale.x;
             y *= kscale.y;
@@ -486,9 +554,9 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
       if constexpr (S::I8) {
 #pragma unroll
         for (int j = 0; j < KT / 8; ++j) {
-          const uint2 w = lds8(base + S::SCALES + KT * 4 + (8 * j + 2 * t) * 4);
-          vs[j][0] = __uint_as_float(w.x);
-          vs[j][1] = __uint_as_float(w.y);
+          const float2 w = *reinterpret_cast<const float2*>(sc + KT + 8 * j + 2 * t);
+          vs[j][0] = w.x;
+          vs[j][1] = w.y;
           vtop = fmaxf(vtop, fmaxf(fabsf(vs[j][0]), fabsf(vs[j][1])));
         }
         vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
@@ -561,48 +629,32 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
           }
         }
       };
+      // 32 bytes of 16 value rows at a time, transposed: lane l reads row l % 16, piece l / 16
 #pragma unroll
-      for (int kk = 0; kk < KT / 16; ++kk) {
+      for (int kk = 0; kk < KT / 16; ++kk)
 #pragma unroll
-        for (int sg = 0; sg < S::VSEG; ++sg) {
-          uint32_t w[4][S::VB / 4];
+        for (int q = 0; q < S::RB / 32; ++q) {
+          const uint4 w = ldmatrix4<true>(vbase + (q * 32 / S::SUB * KT + 16 * kk) * S::SUB +
+                                          (q * 32 % S::SUB ^ v_lane));
+          if constexpr (S::I8) {
+            // a register holds elements 2 g, 2 g + 1 of position 2 t, then of 2 t + 1
+            const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const uint32_t p = base + S::KBYTES + ((kk * 4 + r) * S::VSEG + sg) * 32 * S::VB + lane * S::VB;
-            if constexpr (S::VB == 16) {
-              const uint4 x = lds16(p);
-              w[r][0] = x.x, w[r][1] = x.y, w[r][2] = x.z, w[r][3] = x.w;
-            } else {
-              const uint2 x = lds8(p);
-              w[r][0] = x.x, w[r][1] = x.y;
+            for (int h = 0; h < 2; ++h) {
+              mma_pv(kk, 4 * q + 2 * h, bytes_to_half2(u[2 * h], 0x4240), bytes_to_half2(u[2 * h + 1], 0x4240));
+              mma_pv(kk, 4 * q + 2 * h + 1, bytes_to_half2(u[2 * h], 0x4341), bytes_to_half2(u[2 * h + 1], 0x4341));
             }
-          }
-#pragma unroll
-          for (int i4 = 0; i4 < S::VB / 4; ++i4) {
-            if constexpr (S::I8) {
-#pragma unroll
-              for (int r = 0; r < 4; ++r) w[r][i4] ^= 0x80808080u;
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {  // bytes 2 h, 2 h + 1 of the rows' words, paired by position
-                const uint32_t lo = __byte_perm(w[0][i4], w[1][i4], h ? 0x7362 : 0x5140);
-                const uint32_t hi = __byte_perm(w[2][i4], w[3][i4], h ? 0x7362 : 0x5140);
-                const int n = sg * S::CH + 4 * i4 + 2 * h;
-                mma_pv(kk, n, bytes_to_half2(lo, 0x4140), bytes_to_half2(hi, 0x4140));
-                mma_pv(kk, n + 1, bytes_to_half2(lo, 0x4342), bytes_to_half2(hi, 0x4342));
-              }
-            } else {
-              const int n = sg * S::CH + 2 * i4;
-              mma_pv(kk, n, __byte_perm(w[0][i4], w[1][i4], 0x5410), __byte_perm(w[2][i4], w[3][i4], 0x5410));
-              mma_pv(kk, n + 1, __byte_perm(w[0][i4], w[1][i4], 0x7632), __byte_perm(w[2][i4], w[3][i4], 0x7632));
-            }
+          } else {
+            mma_pv(kk, 2 * q, w.x, w.y);
+            mma_pv(kk, 2 * q + 1, w.z, w.w);
           }
         }
-      }
     }
 
     // ---- the item's (or the stretch's) last round: join the warps
     if (use.rd + 1 == use.units || i + 1 == n_units) {
-      float* part = reinterpret_cast<float*>(smem + (warp * S::STAGES + stage) * S::STAGE);
+      float* part = reinterpret_cast<float*>(ring + stage * S::STAGE);
+      float* stats = reinterpret_cast<float*>(smem + S::STATS);  // [warp][m, l][head]
       __syncwarp();  // the stage's tile has been read by all lanes
       const float vback = S::I8 ? vu : 1.0f;
 #pragma unroll
@@ -611,22 +663,26 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
         l[mt] += __shfl_xor_sync(0xffffffffu, l[mt], 2);
         const int h = mt * 8 + g;
         if (t == 0) {
-          part[S::HEADS * S::PITCH + h] = m[mt];
-          part[S::HEADS * S::PITCH + S::HEADS + h] = l[mt];
+          stats[(warp * 2) * S::HEADS + h] = m[mt];
+          stats[(warp * 2 + 1) * S::HEADS + h] = l[mt];
         }
+        // element d of head h at d ^ 8 (h % 8): the lanes of a store spread over the banks
+        float* row = part + h * D;
+        const int turn = 8 * g;
 #pragma unroll
-        for (int sg = 0; sg < S::VSEG; ++sg)
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int e = 0; e < S::CH; e += 4) {
-              float4 v;
-              v.x = (o[mt][sg * S::CH + e][c] + o[mt][sg * S::CH + e][c + 2]) * vback;
-              v.y = (o[mt][sg * S::CH + e + 1][c] + o[mt][sg * S::CH + e + 1][c + 2]) * vback;
-              v.z = (o[mt][sg * S::CH + e + 2][c] + o[mt][sg * S::CH + e + 2][c + 2]) * vback;
-              v.w = (o[mt][sg * S::CH + e + 3][c] + o[mt][sg * S::CH + e + 3][c + 2]) * vback;
-              *reinterpret_cast<float4*>(part + h * S::PITCH + sg * 8 * S::CH + (2 * t + c) * S::CH + e) = v;
-            }
+        for (int n = 0; n < D / 8; n += S::I8 ? 2 : 1) {
+          if constexpr (S::I8) {
+            float4 v;
+            v.x = (o[mt][n][0] + o[mt][n][2]) * vback;
+            v.y = (o[mt][n + 1][0] + o[mt][n + 1][2]) * vback;
+            v.z = (o[mt][n][1] + o[mt][n][3]) * vback;
+            v.w = (o[mt][n + 1][1] + o[mt][n + 1][3]) * vback;
+            *reinterpret_cast<float4*>(row + ((8 * n + 4 * t) ^ turn)) = v;
+          } else {
+            *reinterpret_cast<float2*>(row + ((8 * n + 2 * t) ^ turn)) =
+                make_float2(o[mt][n][0] + o[mt][n][2], o[mt][n][1] + o[mt][n][3]);
+          }
+        }
       }
       __syncthreads();
       const int kvh = use.it / a.blocks, hb = use.it % a.blocks;
@@ -642,15 +698,15 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
         float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          pm[w] = reinterpret_cast<const float*>(smem + (w * S::STAGES + stage) * S::STAGE)[S::HEADS * S::PITCH + h];
+          pm[w] = stats[(w * 2) * S::HEADS + h];
           M = fmaxf(M, pm[w]);
         }
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
           const float* p = reinterpret_cast<const float*>(smem + (w * S::STAGES + stage) * S::STAGE);
           const float f = pm[w] == -INFINITY ? 0.0f : exp2_approx(pm[w] - M);
-          const float4 y = *reinterpret_cast<const float4*>(p + h * S::PITCH + d);
-          L += f * p[S::HEADS * S::PITCH + S::HEADS + h];
+          const float4 y = *reinterpret_cast<const float4*>(p + h * D + (d ^ (8 * (h & 7))));
+          L += f * stats[(w * 2 + 1) * S::HEADS + h];
           v.x += f * y.x;
           v.y += f * y.y;
           v.z += f * y.z;
@@ -684,18 +740,35 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
             const int h = x / D, d = x % D;
             float M = -INFINITY, L = 0.0f;
             float4 v = make_float4(0, 0, 0, 0);
-            for (int b = c0; b <= c1; ++b) {
-              const float* p = a.records + (static_cast<int64_t>(b) * 2 + (b == c0)) * S::RECORD;
-              const float4 y = __ldcg(reinterpret_cast<const float4*>(p + h * D + d));
-              const float bm = __ldcg(p + S::HEADS * D + h), bl = __ldcg(p + S::HEADS * D + S::HEADS + h);
-              const float nm = fmaxf(M, bm);
+            constexpr int B = 8;  // records in flight
+            for (int b0 = c0; b0 <= c1; b0 += B) {
+              float4 y[B];
+              float bm[B], bl[B];
+#pragma unroll
+              for (int b = 0; b < B; ++b) {
+                const int at = min(b0 + b, c1);
+                const float* p = a.records + (static_cast<int64_t>(at) * 2 + (at == c0)) * S::RECORD;
+                y[b] = __ldcg(reinterpret_cast<const float4*>(p + h * D + d));
+                bm[b] = __ldcg(p + S::HEADS * D + h);
+                bl[b] = __ldcg(p + S::HEADS * D + S::HEADS + h);
+              }
+              float nm = M;
+#pragma unroll
+              for (int b = 0; b < B; ++b) {
+                if (b0 + b > c1) bm[b] = -INFINITY, bl[b] = 0.0f, y[b] = make_float4(0, 0, 0, 0);
+                nm = fmaxf(nm, bm[b]);
+              }
               const float f = M == -INFINITY ? 0.0f : exp2_approx(M - nm);
-              const float e = bm == -INFINITY ? 0.0f : exp2_approx(bm - nm);
-              L = L * f + bl * e;
-              v.x = v.x * f + y.x * e;
-              v.y = v.y * f + y.y * e;
-              v.z = v.z * f + y.z * e;
-              v.w = v.w * f + y.w * e;
+              L *= f, v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+#pragma unroll
+              for (int b = 0; b < B; ++b) {
+                const float e = bm[b] == -INFINITY ? 0.0f : exp2_approx(bm[b] - nm);
+                L += bl[b] * e;
+                v.x += y[b].x * e;
+                v.y += y[b].y * e;
+                v.z += y[b].z * e;
+                v.w += y[b].w * e;
+              }
               M = nm;
             }
             const bool empty = M == -INFINITY && L == 0.0f;
@@ -705,16 +778,26 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS) attend_kernel(const __gr
           }
         }
       }
+      fence_proxy_async_smem();
       __syncthreads();  // the stages that held the partial results may be refilled
       fresh = true;
     }
     use.next<UNIT>(a, items);
+    if (++stage == S::STAGES) {
+      stage = 0;
+      phase ^= 1;
+    }
   }
+  if (late)  // copies still under way must not land after the CTA has gone
+    for (int s = 0; s < S::STAGES && s < n_units; ++s) {
+      const int uses = (n_units - 1 - s) / S::STAGES;
+      mbar_wait_err(bars + s, uses & 1, 2u, &g_paged_error);
+    }
   zero_empty_rows<D>(a);
 }
 
 template <typename S>
-tl_status attend_launch(const AttendArgs& a, cudaStream_t s) {
+tl_status attend_launch(AttendArgs& a, cudaStream_t s) {
   // the line of units has 31 bits
   const int64_t most = static_cast<int64_t>(a.c.hkv) * a.blocks *
                        ((static_cast<int64_t>(a.c.max_pages) * a.c.ps + S::UNIT - 1) / S::UNIT);
@@ -730,7 +813,13 @@ tl_status attend_launch(const AttendArgs& a, cudaStream_t s) {
   }
   // as many CTAs as the device holds at once, fewer where the table has no room for so many rounds
   const int64_t grid = std::min<int64_t>(most * a.rows, std::min(kMaxCtas, device_sm_count() * S::CTAS));
-  attend_kernel<S><<<static_cast<unsigned>(grid), kWarps * 32, S::SMEM, s>>>(a);
+  a.box = std::gcd(a.c.ps, S::KT);
+  CUtensorMap tm_k, tm_v;
+  const long long pool_rows = static_cast<long long>(a.c.pages) * a.c.hkv * a.c.ps;
+  if (tc_encode_rows_bytes(&tm_k, a.c.k, pool_rows, S::RB, a.box) != cudaSuccess ||
+      tc_encode_rows_bytes(&tm_v, a.c.v, pool_rows, S::RB, a.box) != cudaSuccess)
+    return TL_ERR_CUDA;
+  attend_kernel<S><<<static_cast<unsigned>(grid), kWarps * 32, S::SMEM, s>>>(a, tm_k, tm_v);
   return cuda_status(cudaGetLastError());
 }
 
@@ -755,6 +844,14 @@ tl_status attend_dim(AttendArgs& a, int d, cudaStream_t s) {
 constexpr size_t kTicketBytes = (kMaxCtas * sizeof(unsigned int) + 255) / 256 * 256;
 
 }  // namespace
+
+cudaError_t paged_attn_read_error(unsigned int* code) {
+  const cudaError_t e = cudaMemcpyFromSymbol(code, g_paged_error, sizeof(unsigned int));
+  if (e != cudaSuccess || !*code) return e;
+  const unsigned int zero = 0;
+  return cudaMemcpyToSymbol(g_paged_error, &zero, sizeof(unsigned int));
+}
+
 }  // namespace tl
 
 using namespace tl;
