@@ -46,7 +46,7 @@ namespace {
 #define VAR_S128 3
 #endif
 #ifndef VAR_S256
-#define VAR_S256 3
+#define VAR_S256 2
 #endif
 #ifndef VAR_C64
 #define VAR_C64 3
@@ -98,6 +98,9 @@ TL_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memor
 template <int N>
 TL_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+TL_DEV void prefetch_tensormap(const CUtensorMap* tm) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(tm)) : "memory");
+}
 // Four 8x8 matrices of 16-bit elements, lane l's address naming row l % 8 of
 // matrix l / 8; TRANS transposes each.
 template <bool TRANS>
@@ -171,12 +174,16 @@ struct Shape {
   static constexpr int STAGE = 2 * HALF;
   static_assert(MERGE <= STAGE && STAGE % 1024 == 0 && (KT * SUB) % 1024 == 0, "swizzled boxes, partial results");
   static constexpr int STAGES = RB == 64 ? VAR_S64 : RB == 128 ? VAR_S128 : VAR_S256;
-  // shared memory: rings, then scales (int8), tile masks, partial m and l, barriers
+  // shared memory: rings, the query's parts, then scales (int8), tile masks, partial m and l, query scales, barriers
   static constexpr int RING = kWarps * STAGES * STAGE;
-  static constexpr int SCALES = RING;
+  static constexpr int QROW = D * 2;                    // bytes of a query row in 16 bits
+  static constexpr int QTILE = 16 * QROW, QTHIRD = PARTS == 3 ? 8 * QROW : 0;
+  static constexpr int QUERY = RING;                    // [m tile]: 16 rows (8 high, 8 low), then 8 third rows
+  static constexpr int SCALES = QUERY + MT * (QTILE + QTHIRD);
   static constexpr int MASKS = SCALES + (I8 ? kWarps * STAGES * 2 * KT * 4 : 0);
   static constexpr int STATS = MASKS + kWarps * STAGES * 4;
-  static constexpr int BARS = (STATS + kWarps * 2 * HEADS * 4 + 7) / 8 * 8;
+  static constexpr int QSCALE = STATS + kWarps * 2 * HEADS * 4;
+  static constexpr int BARS = (QSCALE + HEADS * 4 + 7) / 8 * 8;
   static constexpr int SMEM = BARS + kWarps * STAGES * 8 + 1024;  // the base is rounded up to 1024
   static constexpr int UNIT = kWarps * KT;              // positions of one CTA round
   static constexpr int RECORD = HEADS * (D + 2);        // floats of a partial result in the workspace
@@ -185,11 +192,10 @@ struct Shape {
 
 // Length of row r in positions, 0 for rows that name no sequence.
 TL_DEV int row_length(const AttendArgs& a, int r, int* seq) {
+  const int n = a.lengths[r];  // both loads at once
   const int s = a.seq ? a.seq[r] : r;
   *seq = s;
-  int n = (s < 0 || s >= a.c.n_seqs) ? 0 : a.lengths[r];
-  n = min(n, a.c.max_pages * a.c.ps);
-  return max(n, 0);
+  return s < 0 || s >= a.c.n_seqs ? 0 : max(0, min(n, a.c.max_pages * a.c.ps));
 }
 
 // A place in the sequence of units: row r with `units` rounds an item, item
@@ -231,11 +237,18 @@ TL_DEV void store_out(void* out, int dt, int64_t i, float4 v) {
         make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
   }
 }
-TL_DEV float2 load_act2(const void* p, int dt, int64_t i) {
-  if (dt == TL_F32) return *reinterpret_cast<const float2*>(static_cast<const float*>(p) + i);
-  if (dt == TL_BF16)
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(static_cast<const __nv_bfloat16*>(p) + i));
-  return __half22float2(*reinterpret_cast<const __half2*>(static_cast<const __half*>(p) + i));
+TL_DEV float4 load_act4(const void* p, int dt, int64_t i) {
+  if (dt == TL_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+  const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+  float2 x, y;
+  if (dt == TL_BF16) {
+    x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x));
+    y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
+  } else {
+    x = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
+    y = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+  }
+  return make_float4(x.x, x.y, y.x, y.y);
 }
 
 // Rows without positions are on nobody's line: zeros and -infinity.
@@ -267,19 +280,26 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ int sh_units[kWarps];
-  __shared__ int sh_first[2];  // first row of the stretch, units before it
+  __shared__ int4 sh_first;  // the stretch's first row, the units before it, the row's sequence and length
   __shared__ int sh_last;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int items = a.c.hkv * a.blocks;
 
+  if (tid == 0) {
+    prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
+  }
   // ---- the CTA's stretch [u0, u1) of the line
-  int mine = 0;  // units: the launch keeps their number within 31 bits
+  const int ctas = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
   const int per = (a.rows + kWarps * 32 - 1) / (kWarps * 32);
   const int r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
+  int mine = 0;  // units: the launch keeps their number within 31 bits
+  int seq = -1, len = 0;
+  bool empty_row = false;  // a row without positions that this CTA writes
   for (int r = r0; r < r1; ++r) {
-    int s;
-    const int len = row_length(a, r, &s);
+    len = row_length(a, r, &seq);
     mine += (len + UNIT - 1) / UNIT;
+    if (len == 0) empty_row |= r % ctas == cta;
   }
   mine *= items;
   int before = mine;
@@ -289,40 +309,86 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
     if (lane >= o) before += v;
   }
   if (lane == 31) sh_units[warp] = before;
-  __syncthreads();
+  empty_row = __syncthreads_or(empty_row);
   int total = 0;
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += sh_units[w];
     total += sh_units[w];
   }
   before -= mine;
-  const int ctas = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
   const int chunk = static_cast<int>((total + static_cast<unsigned>(ctas) - 1) / ctas);
   const int u0 = static_cast<int>(min(static_cast<int64_t>(cta) * chunk, static_cast<int64_t>(total)));
   const int u1 = static_cast<int>(min(static_cast<int64_t>(u0) + chunk, static_cast<int64_t>(total)));
   if (u0 == u1) {
-    zero_empty_rows<D>(a);
+    if (empty_row) zero_empty_rows<D>(a);
     return;
   }
   if (before <= u0 && u0 < before + mine) {
     int r = r0;
-    int at = before;
-    for (;; ++r) {
-      int s;
-      const int n = (row_length(a, r, &s) + UNIT - 1) / UNIT * items;
-      if (u0 < at + n) break;
-      at += n;
+    for (; per > 1; ++r) {
+      len = row_length(a, r, &seq);
+      const int n = (len + UNIT - 1) / UNIT * items;
+      if (u0 < before + n) break;
+      before += n;
     }
-    sh_first[0] = r;
-    sh_first[1] = at;
+    sh_first = make_int4(r, before, seq, len);
   }
   __syncthreads();
   const int n_units = u1 - u0;
   Place use;
-  use.row<UNIT>(a, sh_first[0]);
-  use.it = (u0 - sh_first[1]) / use.units;
-  use.rd = (u0 - sh_first[1]) % use.units;
+  use.r = sh_first.x;
+  use.seq = sh_first.z;
+  use.len = sh_first.w;
+  use.units = (use.len + UNIT - 1) / UNIT;
+  use.it = (u0 - sh_first.y) / use.units;
+  use.rd = (u0 - sh_first.y) - use.it * use.units;
   Place fill = use;
+
+  // The query of the item at `p`: kQ consecutive elements a thread, first as
+  // loaded, then as 16-bit parts in shared memory.
+  constexpr int kQ = S::HEADS * D / (kWarps * 32), kLanes = D / kQ;  // elements of a thread, threads of a head
+  const int qh = tid / kLanes, qd = tid % kLanes * kQ;
+  float x[kQ];
+  auto load_query = [&](const Place& p) {
+    const int kvh = p.it / a.blocks, hb = p.it - kvh * a.blocks;
+    const bool live = hb * S::HEADS + qh < a.group;
+    const int64_t base = p.r * a.ldq + static_cast<int64_t>(kvh * a.group + (live ? hb * S::HEADS + qh : 0)) * D + qd;
+#pragma unroll
+    for (int e = 0; e < kQ; e += 4) {
+      const float4 y = live ? load_act4(a.q, a.q_dtype, base + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      x[e] = y.x, x[e + 1] = y.y, x[e + 2] = y.z, x[e + 3] = y.w;
+    }
+  };
+  auto store_query = [&]() {
+    float f = 1.0f, back = a.scale * kLog2e;
+    if constexpr (!S::BF) {
+      // a power of two that takes the row's largest element to [2^10, 2^11)
+      float top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kQ; ++e) top = fmaxf(top, fabsf(x[e]));
+#pragma unroll
+      for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const int sh = max(-120, min(120, 10 - (static_cast<int>(__float_as_uint(top) >> 23) - 127)));
+      f = __int_as_float((127 + sh) << 23);
+      back *= __int_as_float((127 - sh) << 23);
+    }
+    if (qd == 0) reinterpret_cast<float*>(smem + S::QSCALE)[qh] = back;
+    unsigned char* tile = smem + S::QUERY + (qh >> 3) * (S::QTILE + S::QTHIRD);
+    const int row = qh & 7;
+#pragma unroll
+    for (int e = 0; e < kQ; e += 2) {
+      // column of the pair (d, d + 1): int8 keys bring elements 4 t .. 4 t + 3 to one lane
+      const int d = qd + e, j = d & 15;
+      const int col = S::I8 ? (d & ~15) + (j & 2) * 4 + (j >> 2) * 2 : d;
+      const int at = (((col >> 3) ^ row) << 4) + (col & 7) * 2;  // 16-byte pieces turned by the row
+      float u = x[e] * f, v = x[e + 1] * f;
+      *reinterpret_cast<uint32_t*>(tile + row * S::QROW + at) = split<S::BF>(u, v);
+      *reinterpret_cast<uint32_t*>(tile + (row + 8) * S::QROW + at) = split<S::BF>(u, v);
+      if constexpr (S::PARTS == 3)
+        *reinterpret_cast<uint32_t*>(tile + S::QTILE + row * S::QROW + at) = split<S::BF>(u, v);
+    }
+  };
+  load_query(use);
 
   // ---- the warp's ring
   unsigned char* ring = smem + warp * S::STAGES * S::STAGE;
@@ -385,28 +451,42 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
       }
     }
   };
-  int filled = 0;
+  // the first tiles' pages are looked up together, then their copies start
+  int filled = 0, next_row = -1;
+  {
+    int rows[S::STAGES];
 #pragma unroll
-  for (int i = 0; i < S::STAGES - 1; ++i) {
-    if (filled < n_units) {
-      copy_tile(i, lookup(fill));
-      fill.next<UNIT>(a, items);
-      ++filled;
+    for (int i = 0; i < S::STAGES; ++i) {
+      rows[i] = -1;
+      if (i < n_units) {
+        rows[i] = lookup(fill);
+        if (i < S::STAGES - 1) fill.next<UNIT>(a, items);
+      }
     }
-    if constexpr (S::I8) cp_async_commit();
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; ++i) {
+      if (filled < n_units) {
+        copy_tile(i, rows[i]);
+        ++filled;
+      }
+      if constexpr (S::I8) cp_async_commit();
+    }
+    next_row = rows[S::STAGES - 1];
   }
-  int next_row = filled < n_units ? lookup(fill) : -1;
+  store_query();
+  __syncthreads();
 
   // Byte offsets of this lane's ldmatrix rows, swizzled: 16-byte piece c of row
   // r of a box lies at piece c ^ (r % 8) of 128-byte rows, c ^ (r / 2 % 4) of
   // 64-byte rows. Row offsets that are multiples of 8 leave the swizzle alone.
   const int l8 = lane & 7, v_row = lane & 15;
+  const uint32_t q32 = smem_u32(smem + S::QUERY);
+  // matrices of a query ldmatrix: rows 0-7, 8-15 of piece 2 k, then of piece 2 k + 1
+  const uint32_t q_row = q32 + v_row * S::QROW, q_piece = (lane >> 4) ^ l8;
   const uint32_t k_lane = l8 * S::SUB + (((lane >> 3) ^ (S::SUB == 128 ? l8 : l8 >> 1)) << 4);
   const uint32_t v_lane = v_row * S::SUB + (((lane >> 4) ^ (S::SUB == 128 ? l8 : l8 >> 1)) << 4);
 
   // ---- the running state of one item
-  uint32_t qa[MT][S::KS][4];                       // query, high and low rows
-  uint32_t qc[S::PARTS == 3 ? MT : 1][S::KS][2];   // third part
   float qscale[MT];
   float o[MT][D / 8][4];
   float m[MT], l[MT];
@@ -416,44 +496,9 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
   for (int i = 0, stage = 0, phase = 0; i < n_units; ++i) {
     if (fresh) {
       fresh = false;
-      const int kvh = use.it / a.blocks, hb = use.it % a.blocks;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const int hg = hb * S::HEADS + mt * 8 + g;
-        const bool live = hg < a.group;
-        const int64_t base = use.r * a.ldq + static_cast<int64_t>(kvh * a.group + (live ? hg : 0)) * D;
-        float x[D / 4];
-        float top = 0.0f;
-#pragma unroll
-        for (int e = 0; e < D / 4; e += 2) {
-          // the elements that the key fragments hold for this lane
-          const int d = e / 4 * 16 + (S::I8 ? t * 4 + e % 4 : t * 2 + e % 4 * 4);
-          const float2 y = live ? load_act2(a.q, a.q_dtype, base + d) : make_float2(0.0f, 0.0f);
-          x[e] = y.x;
-          x[e + 1] = y.y;
-          top = fmaxf(top, fmaxf(fabsf(y.x), fabsf(y.y)));
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        float f = 1.0f;
-        qscale[mt] = a.scale * kLog2e;
-        if constexpr (!S::BF) {
-          // a power of two that takes the row's largest element to [2^10, 2^11)
-          const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-          const int sh = max(-120, min(120, 10 - e));
-          f = __int_as_float((127 + sh) << 23);
-          qscale[mt] = (a.scale * kLog2e) * __int_as_float((127 - sh) << 23);
-        }
-#pragma unroll
-        for (int k = 0; k < S::KS; ++k) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float u = x[k * 4 + h * 2] * f, v = x[k * 4 + h * 2 + 1] * f;
-            qa[mt][k][2 * h] = split<S::BF>(u, v);
-            qa[mt][k][2 * h + 1] = split<S::BF>(u, v);
-            if constexpr (S::PARTS == 3) qc[mt][k][h] = split<S::BF>(u, v);
-          }
-        }
+        qscale[mt] = reinterpret_cast<const float*>(smem + S::QSCALE)[mt * 8 + g];
         m[mt] = -INFINITY;
         l[mt] = 0.0f;
 #pragma unroll
@@ -502,14 +547,29 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
         for (int mt = 0; mt < MT; ++mt) c[j][mt][0] = c[j][mt][1] = c[j][mt][2] = c[j][mt][3] = 0.0f;
       // 64 bytes of a key row at a time: lane l reads row l % 8, piece l / 8
 #pragma unroll
-      for (int q = 0; q < S::RB / 64; ++q)
+      for (int q = 0; q < S::RB / 64; ++q) {
+        uint4 w[KT / 8];
 #pragma unroll
-        for (int j = 0; j < KT / 8; ++j) {
-          const uint4 w = ldmatrix4<false>(kbase + (q * 64 / S::SUB * KT + 8 * j) * S::SUB +
-                                           (q * 64 % S::SUB ^ k_lane));
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+        for (int j = 0; j < KT / 8; ++j)
+          w[j] = ldmatrix4<false>(kbase + (q * 64 / S::SUB * KT + 8 * j) * S::SUB + (q * 64 % S::SUB ^ k_lane));
 #pragma unroll
-          for (int k = 0; k < (S::I8 ? 4 : 2); ++k) {
+        for (int k = 0; k < (S::I8 ? 4 : 2); ++k) {
+          const int ks = q * (S::I8 ? 4 : 2) + k;
+          uint32_t qa[MT][4], third[S::PARTS == 3 ? MT : 1][4];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const uint32_t at = mt * (S::QTILE + S::QTHIRD) + (((2 * ks) ^ q_piece) << 4);
+            const uint4 y = ldmatrix4<false>(q_row + at);
+            qa[mt][0] = y.x, qa[mt][1] = y.y, qa[mt][2] = y.z, qa[mt][3] = y.w;
+            if constexpr (S::PARTS == 3) {
+              // rows 0-7 only: matrices 1 and 3 repeat 0 and 2 and are not used
+              const uint4 z = ldmatrix4<false>(q32 + S::QTILE + l8 * S::QROW + at);
+              third[mt][0] = z.x, third[mt][1] = 0u, third[mt][2] = z.z, third[mt][3] = 0u;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < KT / 8; ++j) {
+            const uint32_t ww[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
             uint32_t b0, b1;
             if constexpr (S::I8) {
               const uint32_t u = ww[k] ^ 0x80808080u;
@@ -519,17 +579,14 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
               b0 = ww[2 * k];
               b1 = ww[2 * k + 1];
             }
-            const int ks = q * (S::I8 ? 4 : 2) + k;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              mma16<S::BF>(c[j][mt], qa[mt][ks], b0, b1);
-              if constexpr (S::PARTS == 3) {
-                const uint32_t third[4] = {qc[mt][ks][0], 0u, qc[mt][ks][1], 0u};
-                mma16<S::BF>(c[j][mt], third, b0, b1);
-              }
+              mma16<S::BF>(c[j][mt], qa[mt], b0, b1);
+              if constexpr (S::PARTS == 3) mma16<S::BF>(c[j][mt], third[mt], b0, b1);
             }
           }
         }
+      }
 #pragma unroll
       for (int j = 0; j < KT / 8; ++j) {
         float2 kscale = make_float2(1.0f, 1.0f);
@@ -684,15 +741,19 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
           }
         }
       }
+      // the next item's query arrives while this one is joined
+      const Place done = use;
+      use.next<UNIT>(a, items);
+      if (i + 1 < n_units) load_query(use);
       __syncthreads();
-      const int kvh = use.it / a.blocks, hb = use.it % a.blocks;
+      const int kvh = done.it / a.blocks, hb = done.it - kvh * a.blocks;
       const int nh = min(S::HEADS, a.group - hb * S::HEADS);
-      const int first = u0 + i - use.rd;  // the item's first unit on the line
-      const int c0 = first / chunk, c1 = (first + use.units - 1) / chunk;
+      const int first = u0 + i - done.rd;  // the item's first unit on the line
+      const int c0 = first / chunk, c1 = (first + done.units - 1) / chunk;
       const bool whole = c0 == c1;
-      const int64_t head0 = static_cast<int64_t>(use.r) * a.heads + kvh * a.group + hb * S::HEADS;
+      const int64_t head0 = static_cast<int64_t>(done.r) * a.heads + kvh * a.group + hb * S::HEADS;
       float* rec = a.records + (static_cast<int64_t>(cta) * 2 + (cta == c0)) * S::RECORD;
-      for (int x = tid * 4; x < nh * D; x += kWarps * 128) {
+      for (int x = tid * 4; x < (whole ? nh : S::HEADS) * D; x += kWarps * 128) {
         const int h = x / D, d = x % D;
         float M = -INFINITY, L = 0.0f, pm[kWarps];
         float4 v = make_float4(0, 0, 0, 0);
@@ -736,53 +797,97 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
         __syncthreads();
         if (sh_last) {
           __threadfence();
-          for (int x = tid * 4; x < nh * D; x += kWarps * 128) {
-            const int h = x / D, d = x % D;
-            float M = -INFINITY, L = 0.0f;
-            float4 v = make_float4(0, 0, 0, 0);
-            constexpr int B = 8;  // records in flight
-            for (int b0 = c0; b0 <= c1; b0 += B) {
-              float4 y[B];
-              float bm[B], bl[B];
+          // A batch's maxima and sums go to shared memory, a warp a head turns
+          // them into weights, then every thread sums its columns.
+          constexpr int COLS = S::HEADS * D / (kWarps * 128), BATCH = 32, DEPTH = 16 / COLS;
+          float* bm = reinterpret_cast<float*>(smem + stage * S::STAGE);  // [head][record]: weights
+          float* top = reinterpret_cast<float*>(smem + S::STATS);  // [head]: maximum, sum, factor of the old sums
+          float* sum = top + S::HEADS;
+          float* old = sum + S::HEADS;
+          float4 v[COLS];
 #pragma unroll
-              for (int b = 0; b < B; ++b) {
-                const int at = min(b0 + b, c1);
-                const float* p = a.records + (static_cast<int64_t>(at) * 2 + (at == c0)) * S::RECORD;
-                y[b] = __ldcg(reinterpret_cast<const float4*>(p + h * D + d));
-                bm[b] = __ldcg(p + S::HEADS * D + h);
-                bl[b] = __ldcg(p + S::HEADS * D + S::HEADS + h);
-              }
-              float nm = M;
+          for (int c = 0; c < COLS; ++c) v[c] = make_float4(0, 0, 0, 0);
+          __syncthreads();
+          if (tid < S::HEADS) {
+            top[tid] = -INFINITY;
+            sum[tid] = 0.0f;
+          }
+          for (int b0 = c0; b0 <= c1; b0 += BATCH) {
+            const int n = min(BATCH, c1 + 1 - b0);
+            // lane = record, warp w takes heads w, w + 4, ...
+            float rm[S::HEADS / kWarps], rl[S::HEADS / kWarps];
 #pragma unroll
-              for (int b = 0; b < B; ++b) {
-                if (b0 + b > c1) bm[b] = -INFINITY, bl[b] = 0.0f, y[b] = make_float4(0, 0, 0, 0);
-                nm = fmaxf(nm, bm[b]);
-              }
-              const float f = M == -INFINITY ? 0.0f : exp2_approx(M - nm);
-              L *= f, v.x *= f, v.y *= f, v.z *= f, v.w *= f;
-#pragma unroll
-              for (int b = 0; b < B; ++b) {
-                const float e = bm[b] == -INFINITY ? 0.0f : exp2_approx(bm[b] - nm);
-                L += bl[b] * e;
-                v.x += y[b].x * e;
-                v.y += y[b].y * e;
-                v.z += y[b].z * e;
-                v.w += y[b].w * e;
-              }
-              M = nm;
+            for (int k = 0; k < S::HEADS / kWarps; ++k) {
+              const int b = b0 + min(lane, n - 1);
+              const float* p = a.records + (static_cast<int64_t>(b) * 2 + (b == c0)) * S::RECORD + S::HEADS * D +
+                               warp + kWarps * k;
+              rm[k] = __ldcg(p);
+              rl[k] = __ldcg(p + S::HEADS);
             }
-            const bool empty = M == -INFINITY && L == 0.0f;
-            const float inv = empty ? 0.0f : 1.0f / L;
-            store_out(a.out, a.q_dtype, (head0 + h) * D + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-            if (a.lse && d == 0) a.lse[head0 + h] = empty ? -INFINITY : (M + log2f(L)) * kLn2;
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < S::HEADS / kWarps; ++k) {
+              const int h = warp + kWarps * k;
+              const float m0 = top[h], m1 = fmaxf(m0, warp_max(rm[k]));
+              const float e = lane >= n || rm[k] == -INFINITY ? 0.0f : exp2_approx(rm[k] - m1);
+              const float l1 = warp_sum(lane < n ? e * rl[k] : 0.0f);
+              bm[h * BATCH + lane] = e;
+              if (lane == 0) {
+                const float f = m0 == -INFINITY ? 0.0f : exp2_approx(m0 - m1);
+                top[h] = m1;
+                sum[h] = sum[h] * f + l1;
+                old[h] = f;
+              }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) {
+              const float f = old[(tid * 4 + c * kWarps * 128) / D];
+              v[c].x *= f, v[c].y *= f, v[c].z *= f, v[c].w *= f;
+            }
+            for (int b1 = 0; b1 < n; b1 += DEPTH) {
+              float4 y[DEPTH][COLS];
+#pragma unroll
+              for (int k = 0; k < DEPTH; ++k) {
+                const int b = b0 + min(b1 + k, n - 1);
+                const float* p = a.records + (static_cast<int64_t>(b) * 2 + (b == c0)) * S::RECORD + tid * 4;
+#pragma unroll
+                for (int c = 0; c < COLS; ++c)
+                  y[k][c] = __ldcg(reinterpret_cast<const float4*>(p + c * kWarps * 128));
+              }
+#pragma unroll
+              for (int k = 0; k < DEPTH; ++k)
+                if (b1 + k < n) {
+#pragma unroll
+                  for (int c = 0; c < COLS; ++c) {
+                    const float e = bm[(tid * 4 + c * kWarps * 128) / D * BATCH + b1 + k];
+                    v[c].x += y[k][c].x * e;
+                    v[c].y += y[k][c].y * e;
+                    v[c].z += y[k][c].z * e;
+                    v[c].w += y[k][c].w * e;
+                  }
+                }
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < COLS; ++c) {
+            const int h = (tid * 4 + c * kWarps * 128) / D, d = (tid * 4) % D;
+            if (h >= nh) continue;
+            const bool empty = top[h] == -INFINITY && sum[h] == 0.0f;
+            const float inv = empty ? 0.0f : 1.0f / sum[h];
+            store_out(a.out, a.q_dtype, (head0 + h) * D + d,
+                      make_float4(v[c].x * inv, v[c].y * inv, v[c].z * inv, v[c].w * inv));
+            if (a.lse && d == 0) a.lse[head0 + h] = empty ? -INFINITY : (top[h] + log2f(sum[h])) * kLn2;
           }
         }
       }
+      if (i + 1 < n_units) store_query();
       fence_proxy_async_smem();
       __syncthreads();  // the stages that held the partial results may be refilled
       fresh = true;
+    } else {
+      use.next<UNIT>(a, items);
     }
-    use.next<UNIT>(a, items);
     if (++stage == S::STAGES) {
       stage = 0;
       phase ^= 1;
@@ -793,7 +898,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
       const int uses = (n_units - 1 - s) / S::STAGES;
       mbar_wait_err(bars + s, uses & 1, 2u, &g_paged_error);
     }
-  zero_empty_rows<D>(a);
+  if (empty_row) zero_empty_rows<D>(a);
 }
 
 template <typename S>
