@@ -35,6 +35,13 @@ tl_status paged_view(const tl_paged_kv* c, const int32_t* table, int32_t n_seqs,
 
 namespace {
 
+// Both kernels move rows and are bound by memory. A row belongs to a few
+// neighbouring threads, each with 16 bytes of it a load, and a thread takes up
+// to kRows rows of one token with all their loads in flight before the first
+// use; the token's angles, sequence and page are looked up meanwhile, once.
+constexpr int kThreads = 256;
+constexpr int kRows = 4;
+
 struct AppendArgs {
   PagedView c;
   const void *q, *k, *v;
@@ -42,153 +49,252 @@ struct AppendArgs {
   const int32_t *seq, *pos;
   const float *cos, *sin;
   int32_t max_pos, tokens, heads;
+  int32_t groups;  // thread groups of a token: each takes rows g, g + groups, ...
   void* q_out;
 };
 
-// One warp per (token, head row): heads query rows, then kv_heads key rows,
-// then kv_heads value rows. Lane l holds the pairs j = l, l + 32 < D / 2.
+// N consecutive elements as float32 and back, in accesses of up to 16 bytes.
+template <typename T, int N>
+TL_DEV void load_n(const T* p, float* x) {
+  constexpr int B = N * sizeof(T);
+  static_assert(B == 4 || B == 8 || B % 16 == 0, "whole accesses");
+  uint32_t w[B / 4];
+  if constexpr (B == 4) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (B == 8) {
+    const uint2 y = *reinterpret_cast<const uint2*>(p);
+    w[0] = y.x, w[1] = y.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < B / 16; ++i) {
+      const uint4 y = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) + 16 * i);
+      w[4 * i] = y.x, w[4 * i + 1] = y.y, w[4 * i + 2] = y.z, w[4 * i + 3] = y.w;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (sizeof(T) == 4)
+      x[i] = __uint_as_float(w[i]);
+    else if constexpr (sizeof(T) == 2)
+      x[i] = to_f32(reinterpret_cast<const T*>(w)[i]);
+    else
+      x[i] = static_cast<float>(static_cast<int8_t>(w[i / 4] >> (8 * (i % 4))));
+  }
+}
+template <typename T, int N>
+TL_DEV void store_n(T* p, const float* x) {
+  constexpr int B = N * sizeof(T);
+  static_assert(B == 8 || B % 16 == 0, "whole accesses");
+  __align__(16) T y[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) y[i] = from_f32<T>(x[i]);
+  if constexpr (B == 8) {
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < B / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(y)[i];
+  }
+}
+
+// Rotation of the pairs (a_i, b_i) = (x_j, x_(j + D/2)) by the token's angles,
+// in float32 without contraction (the INT8 rounding that may follow has to see
+// the reference's values), and quantize_int8 of the whole row, whose maximum
+// is taken over the row's threads. A thread holds N pairs, 16 bytes of each
+// half; D = 64, 32 + 2 * 4 head rows of bfloat16: 10 KB a token moved.
+// Measured: 16384 such tokens (171 MB) {T_PROMPT}, one token {T_ONE}.
 template <typename TI, typename TC, int D>
-__global__ void append_kernel(AppendArgs a) {
-  const int lane = threadIdx.x & 31;
-  const int per = (a.q ? a.heads : 0) + 2 * a.c.hkv;
-  const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  if (w >= static_cast<int64_t>(a.tokens) * per) return;
-  const int t = static_cast<int>(w / per);
-  int h = static_cast<int>(w % per);
-  int kind = 2;  // 0 query, 1 key, 2 value
-  const int hq = a.q ? a.heads : 0;
-  if (h < hq) {
-    kind = 0;
-  } else if (h < hq + a.c.hkv) {
-    kind = 1;
-    h -= hq;
-  } else {
-    h -= hq + a.c.hkv;
+__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int N = 16 / sizeof(TI), LANES = D / 2 / N;  // pairs of a thread, threads of a row
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int j = static_cast<int>(id % LANES) * N;
+  const unsigned part = static_cast<unsigned>(id / LANES);
+  const int64_t t = part / static_cast<unsigned>(a.groups);
+  const int g = static_cast<int>(part - static_cast<unsigned>(t) * a.groups);
+  const bool in = t < a.tokens;  // (the row maxima below are warp-wide)
+  const int rows = a.heads + 2 * a.c.hkv;
+
+  float lo[kRows][N], hi[kRows][N];
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int r = g + u * a.groups;
+    if (!in || r >= rows) continue;
+    const TI* x = r < a.heads ? static_cast<const TI*>(a.q) + t * a.ldq + r * D
+                  : r < a.heads + a.c.hkv
+                      ? static_cast<const TI*>(a.k) + t * a.ldk + (r - a.heads) * D
+                      : static_cast<const TI*>(a.v) + t * a.ldv + (r - a.heads - a.c.hkv) * D;
+    load_n<TI, N>(x + j, lo[u]);
+    load_n<TI, N>(x + j + D / 2, hi[u]);
   }
-  const int p = a.pos[t];
+  const int p = in ? a.pos[t] : -1, s = in ? a.seq[t] : -1;
   const bool angle = !a.cos || (p >= 0 && p < a.max_pos);
-  const TI* src = kind == 0   ? static_cast<const TI*>(a.q) + t * a.ldq
-                  : kind == 1 ? static_cast<const TI*>(a.k) + t * a.ldk
-                              : static_cast<const TI*>(a.v) + t * a.ldv;
-  src += h * D;
-  constexpr int NP = D / 64;
-  float lo[NP], hi[NP];
-#pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int j = lane + 32 * i;
-    lo[i] = to_f32(src[j]);
-    hi[i] = to_f32(src[j + D / 2]);
-    if (kind != 2 && a.cos) {
-      const float cs = angle ? a.cos[static_cast<int64_t>(p) * D + j] : 0.0f;
-      const float sn = angle ? a.sin[static_cast<int64_t>(p) * D + j] : 0.0f;
-      const float x = lo[i], y = hi[i];
-      lo[i] = __fsub_rn(__fmul_rn(x, cs), __fmul_rn(y, sn));
-      hi[i] = __fadd_rn(__fmul_rn(y, cs), __fmul_rn(x, sn));
-    }
+  float cs[N], sn[N];
+  if (a.cos && angle) {
+    load_n<float, N>(a.cos + static_cast<int64_t>(p) * D + j, cs);
+    load_n<float, N>(a.sin + static_cast<int64_t>(p) * D + j, sn);
   }
-  if (kind == 0) {
-    TI* o = static_cast<TI*>(a.q_out) + (static_cast<int64_t>(t) * a.heads + h) * D;
+  const int64_t row0 = angle ? paged_row(a.c, s, p) : -1;
+
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      o[lane + 32 * i] = from_f32<TI>(angle ? lo[i] : 0.0f);
-      o[lane + 32 * i + D / 2] = from_f32<TI>(angle ? hi[i] : 0.0f);
+  for (int u = 0; u < kRows; ++u) {
+    const int r = g + u * a.groups;
+    const bool query = r < a.heads, key = !query && r < a.heads + a.c.hkv;
+    const bool here = in && r < rows;
+    if (here && (query || key) && a.cos && angle) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float x = lo[u][i], y = hi[u][i];
+        lo[u][i] = __fsub_rn(__fmul_rn(x, cs[i]), __fmul_rn(y, sn[i]));
+        hi[u][i] = __fadd_rn(__fmul_rn(y, cs[i]), __fmul_rn(x, sn[i]));
+      }
     }
-    return;
-  }
-  const int64_t row0 = angle ? paged_row(a.c, a.seq[t], p) : -1;
-  if (row0 < 0) return;
-  const int64_t row = row0 + static_cast<int64_t>(h) * a.c.ps;
-  TC* o = static_cast<TC*>(kind == 1 ? a.c.k : a.c.v) + row * D;
-  if constexpr (sizeof(TC) == 1) {
-    float m = 0.0f;
-    bool bad = false;
+    if (here && query) {
+      TI* o = static_cast<TI*>(a.q_out) + (t * a.heads + r) * D + j;
+      if (!angle) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      m = fmaxf(m, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
-      bad |= !isfinite(lo[i]) || !isfinite(hi[i]);
+        for (int i = 0; i < N; ++i) lo[u][i] = hi[u][i] = 0.0f;
+      }
+      store_n<TI, N>(o, lo[u]);
+      store_n<TI, N>(o + D / 2, hi[u]);
     }
-    m = warp_max(m);
-    bad = __any_sync(0xffffffffu, bad);
-    const float sc = bad ? __int_as_float(0x7fc00000) : static_cast<float>(quant_scale64(m));
+    const int64_t row = row0 + static_cast<int64_t>(r - a.heads - (key ? 0 : a.c.hkv)) * a.c.ps;
+    TC* o = static_cast<TC*>(key ? a.c.k : a.c.v) + row * D + j;
+    const bool store = here && !query && row0 >= 0;
+    if constexpr (sizeof(TC) == 1) {
+      if (!__any_sync(0xffffffffu, store)) continue;
+      // the row's maximum; a NaN or an infinity anywhere gives a NaN scale
+      float m = 0.0f;
+      if (store) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      o[lane + 32 * i] = bad ? 0 : static_cast<int8_t>(quantize_one(lo[i], sc));
-      o[lane + 32 * i + D / 2] = bad ? 0 : static_cast<int8_t>(quantize_one(hi[i], sc));
-    }
-    if (lane == 0) (kind == 1 ? a.c.ks : a.c.vs)[row] = sc;
-  } else {
+        for (int i = 0; i < N; ++i) m = fmaxf(m, fmaxf(fabsf(lo[u][i]), fabsf(hi[u][i])));
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      o[lane + 32 * i] = from_f32<TC>(lo[i]);
-      o[lane + 32 * i + D / 2] = from_f32<TC>(hi[i]);
+        for (int i = 0; i < N; ++i)
+          if (lo[u][i] != lo[u][i] || hi[u][i] != hi[u][i]) m = INFINITY;
+      }
+#pragma unroll
+      for (int w = 1; w < LANES; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+      if (store) {
+        const bool bad = m == INFINITY;
+        // absmax / 127 in float64 rounded to float32 is the float32 quotient (53 >= 2 * 24 + 2 bits)
+        const float sc = bad ? __int_as_float(0x7fc00000) : m == 0.0f ? 1.0f : __fdiv_rn(m, 127.0f);
+        const float inv = quant_inv(sc);
+        const bool tiny = inv == INFINITY;  // a scale below 2^-128 has no reciprocal
+        auto quantize = [&](float f) { return (tiny ? quantize_one(f, sc) : quantize_one_inv(f, sc, inv)) & 255; };
+        uint32_t x[N / 4], y[N / 4];
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) x[i] = y[i] = 0;
+        if (!bad) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            x[i / 4] |= quantize(lo[u][i]) << (8 * (i % 4));
+            y[i / 4] |= quantize(hi[u][i]) << (8 * (i % 4));
+          }
+        }
+        if constexpr (N == 4) {
+          *reinterpret_cast<uint32_t*>(o) = x[0];
+          *reinterpret_cast<uint32_t*>(o + D / 2) = y[0];
+        } else {
+          *reinterpret_cast<uint2*>(o) = make_uint2(x[0], x[1]);
+          *reinterpret_cast<uint2*>(o + D / 2) = make_uint2(y[0], y[1]);
+        }
+        if (j == 0) (key ? a.c.ks : a.c.vs)[row] = sc;
+      }
+    } else if (store) {
+      store_n<TC, N>(o, lo[u]);
+      store_n<TC, N>(o + D / 2, hi[u]);
     }
   }
 }
 
-// One warp per (token, kv head) of K, then of V.
+// Rows back as float32 or 16 bits: 16 bytes of output a thread and row.
+// Measured: 28791 tokens of 8 heads of 128 (bfloat16, 236 MB) {T_READ}.
 template <typename TC, typename TO, int D>
-__global__ void read_kernel(PagedView c, const int32_t* seq, const int32_t* pos, int32_t tokens, TO* k_out,
-                            TO* v_out) {
-  const int lane = threadIdx.x & 31;
-  const int64_t w = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  if (w >= static_cast<int64_t>(tokens) * 2 * c.hkv) return;
-  const int t = static_cast<int>(w / (2 * c.hkv));
-  int h = static_cast<int>(w % (2 * c.hkv));
-  const bool key = h < c.hkv;
-  if (!key) h -= c.hkv;
-  TO* o = key ? k_out : v_out;
-  if (!o) return;
-  o += (static_cast<int64_t>(t) * c.hkv + h) * D;
+__global__ void __launch_bounds__(kThreads)
+    read_kernel(const __grid_constant__ PagedView c, const int32_t* seq, const int32_t* pos, int32_t tokens,
+                int32_t groups, TO* k_out, TO* v_out) {
+  constexpr int N = 16 / sizeof(TO), LANES = D / N;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int j = static_cast<int>(id % LANES) * N;
+  const unsigned part = static_cast<unsigned>(id / LANES);
+  const int64_t t = part / static_cast<unsigned>(groups);
+  const int g = static_cast<int>(part - static_cast<unsigned>(t) * groups);
+  if (t >= tokens) return;
   const int64_t row0 = paged_row(c, seq[t], pos[t]);
-  const int64_t row = row0 + static_cast<int64_t>(h) * c.ps;
-  const TC* x = static_cast<const TC*>(key ? c.k : c.v) + row * D;
+  float x[kRows][N], sc[kRows];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    float y = 0.0f;
-    if (row0 >= 0) {
-      if constexpr (sizeof(TC) == 1)
-        y = __fmul_rn(static_cast<float>(x[lane + 32 * i]), (key ? c.ks : c.vs)[row]);
-      else
-        y = to_f32(x[lane + 32 * i]);
+  for (int u = 0; u < kRows; ++u) {
+    const int r = g + u * groups;
+    const bool key = r < c.hkv;
+    const int64_t row = row0 + static_cast<int64_t>(key ? r : r - c.hkv) * c.ps;
+    sc[u] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[u][i] = 0.0f;
+    if (row0 < 0 || r >= 2 * c.hkv || !(key ? k_out : v_out)) continue;
+    load_n<TC, N>(static_cast<const TC*>(key ? c.k : c.v) + row * D + j, x[u]);
+    if constexpr (sizeof(TC) == 1) sc[u] = (key ? c.ks : c.vs)[row];
+  }
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const int r = g + u * groups;
+    TO* o = r < c.hkv ? k_out : v_out;
+    if (r >= 2 * c.hkv || !o) continue;
+    if constexpr (sizeof(TC) == 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[u][i] = __fmul_rn(x[u][i], sc[u]);
     }
-    o[lane + 32 * i] = from_f32<TO>(y);
+    store_n<TO, N>(o + (t * c.hkv + (r < c.hkv ? r : r - c.hkv)) * D + j, x[u]);
   }
 }
 
+// CTAs for `rows` rows of `lanes` threads a token; false if a grid cannot hold them.
+bool grid_for(int tokens, int rows, int lanes, int* groups, unsigned* grid) {
+  *groups = (rows + kRows - 1) / kRows;
+  const int64_t ctas = (static_cast<int64_t>(tokens) * *groups * lanes + kThreads - 1) / kThreads;
+  *grid = static_cast<unsigned>(ctas);
+  return static_cast<int64_t>(tokens) * *groups + kThreads <= INT32_MAX && ctas <= INT32_MAX;
+}
+
+template <typename TI, typename TC, int D>
+tl_status append_launch(AppendArgs& a, cudaStream_t s) {
+  unsigned grid;
+  if (!grid_for(a.tokens, a.heads + 2 * a.c.hkv, D / 2 * sizeof(TI) / 16, &a.groups, &grid)) return TL_ERR_OUT_OF_RANGE;
+  append_kernel<TI, TC, D><<<grid, kThreads, 0, s>>>(a);
+  return cuda_status(cudaGetLastError());
+}
 template <typename TI, typename TC>
-cudaError_t append_launch(const AppendArgs& a, int d, cudaStream_t s) {
-  const int64_t warps = static_cast<int64_t>(a.tokens) * ((a.q ? a.heads : 0) + 2 * a.c.hkv);
-  const unsigned grid = static_cast<unsigned>((warps + 7) / 8);
-  if (d == 64)
-    append_kernel<TI, TC, 64><<<grid, 256, 0, s>>>(a);
-  else
-    append_kernel<TI, TC, 128><<<grid, 256, 0, s>>>(a);
-  return cudaGetLastError();
+tl_status append_dim(AppendArgs& a, int d, cudaStream_t s) {
+  return d == 64 ? append_launch<TI, TC, 64>(a, s) : append_launch<TI, TC, 128>(a, s);
 }
 template <typename TI>
-cudaError_t append_pool(const AppendArgs& a, int pool, int d, cudaStream_t s) {
-  return pool == TL_I8     ? append_launch<TI, int8_t>(a, d, s)
-         : pool == TL_BF16 ? append_launch<TI, __nv_bfloat16>(a, d, s)
-                           : append_launch<TI, __half>(a, d, s);
+tl_status append_pool(AppendArgs& a, int pool, int d, cudaStream_t s) {
+  return pool == TL_I8     ? append_dim<TI, int8_t>(a, d, s)
+         : pool == TL_BF16 ? append_dim<TI, __nv_bfloat16>(a, d, s)
+                           : append_dim<TI, __half>(a, d, s);
 }
 
+struct ReadArgs {
+  PagedView c;
+  const int32_t *seq, *pos;
+  int32_t tokens;
+  void *k, *v;
+};
+template <typename TC, typename TO, int D>
+tl_status read_launch(const ReadArgs& a, cudaStream_t s) {
+  unsigned grid;
+  int groups;
+  if (!grid_for(a.tokens, 2 * a.c.hkv, D * sizeof(TO) / 16, &groups, &grid)) return TL_ERR_OUT_OF_RANGE;
+  read_kernel<TC, TO, D><<<grid, kThreads, 0, s>>>(a.c, a.seq, a.pos, a.tokens, groups, static_cast<TO*>(a.k),
+                                                   static_cast<TO*>(a.v));
+  return cuda_status(cudaGetLastError());
+}
 template <typename TC, typename TO>
-cudaError_t read_launch(const PagedView& c, const int32_t* seq, const int32_t* pos, int tokens, void* k, void* v, int d,
-                        cudaStream_t s) {
-  const int64_t warps = static_cast<int64_t>(tokens) * 2 * c.hkv;
-  const unsigned grid = static_cast<unsigned>((warps + 7) / 8);
-  if (d == 64)
-    read_kernel<TC, TO, 64><<<grid, 256, 0, s>>>(c, seq, pos, tokens, static_cast<TO*>(k), static_cast<TO*>(v));
-  else
-    read_kernel<TC, TO, 128><<<grid, 256, 0, s>>>(c, seq, pos, tokens, static_cast<TO*>(k), static_cast<TO*>(v));
-  return cudaGetLastError();
+tl_status read_dim(const ReadArgs& a, int d, cudaStream_t s) {
+  return d == 64 ? read_launch<TC, TO, 64>(a, s) : read_launch<TC, TO, 128>(a, s);
 }
 template <typename TC>
-cudaError_t read_out(const PagedView& c, const int32_t* seq, const int32_t* pos, int tokens, void* k, void* v, int out,
-                     int d, cudaStream_t s) {
-  return out == TL_F32    ? read_launch<TC, float>(c, seq, pos, tokens, k, v, d, s)
-         : out == TL_BF16 ? read_launch<TC, __nv_bfloat16>(c, seq, pos, tokens, k, v, d, s)
-                          : read_launch<TC, __half>(c, seq, pos, tokens, k, v, d, s);
+tl_status read_out(const ReadArgs& a, int out, int d, cudaStream_t s) {
+  return out == TL_F32    ? read_dim<TC, float>(a, d, s)
+         : out == TL_BF16 ? read_dim<TC, __nv_bfloat16>(a, d, s)
+                          : read_dim<TC, __half>(a, d, s);
 }
 
 }  // namespace
@@ -231,24 +337,29 @@ tl_status tl_paged_append(const tl_paged_kv* cache, const void* q, const void* k
   a.heads = q ? heads : 0;
   a.q_out = q_out;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return cuda_status(dtype == TL_F32    ? append_pool<float>(a, cache->dtype, cache->head_dim, s)
-                     : dtype == TL_BF16 ? append_pool<__nv_bfloat16>(a, cache->dtype, cache->head_dim, s)
-                                        : append_pool<__half>(a, cache->dtype, cache->head_dim, s));
+  return dtype == TL_F32    ? append_pool<float>(a, cache->dtype, cache->head_dim, s)
+         : dtype == TL_BF16 ? append_pool<__nv_bfloat16>(a, cache->dtype, cache->head_dim, s)
+                            : append_pool<__half>(a, cache->dtype, cache->head_dim, s);
 }
 
 tl_status tl_paged_read(const tl_paged_kv* cache, const int32_t* seq, const int32_t* pos, const int32_t* block_table,
                         int32_t n_seqs, int32_t max_pages, int64_t table_stride, int32_t tokens, void* k_out,
                         void* v_out, int32_t out_dtype, void* stream) {
-  PagedView c;
-  const tl_status st = paged_view(cache, block_table, n_seqs, max_pages, table_stride, &c);
+  ReadArgs a;
+  const tl_status st = paged_view(cache, block_table, n_seqs, max_pages, table_stride, &a.c);
   if (st != TL_OK) return st;
   if (!seq || !pos || tokens <= 0 || !is_float_dtype(out_dtype) || (!k_out && !v_out)) return TL_ERR_INVALID_ARGUMENT;
   if (!aligned_to(k_out, 16) || !aligned_to(v_out, 16)) return TL_ERR_INVALID_ARGUMENT;
+  a.seq = seq;
+  a.pos = pos;
+  a.tokens = tokens;
+  a.k = k_out;
+  a.v = v_out;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int d = cache->head_dim;
-  return cuda_status(cache->dtype == TL_I8     ? read_out<int8_t>(c, seq, pos, tokens, k_out, v_out, out_dtype, d, s)
-                     : cache->dtype == TL_BF16 ? read_out<__nv_bfloat16>(c, seq, pos, tokens, k_out, v_out, out_dtype, d, s)
-                                               : read_out<__half>(c, seq, pos, tokens, k_out, v_out, out_dtype, d, s));
+  return cache->dtype == TL_I8     ? read_out<int8_t>(a, out_dtype, d, s)
+         : cache->dtype == TL_BF16 ? read_out<__nv_bfloat16>(a, out_dtype, d, s)
+                                   : read_out<__half>(a, out_dtype, d, s);
 }
 
 }  // extern "C"
