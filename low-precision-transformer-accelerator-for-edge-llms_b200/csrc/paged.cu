@@ -1,5 +1,8 @@
 // paged.cu -- appending rotated keys and values to a paged KV cache and
 // reading rows of it back (tl_paged_append, tl_paged_read).
+#include <type_traits>
+
+#include "kernels.cuh"
 #include "serving.cuh"
 
 namespace tl {
@@ -39,7 +42,7 @@ namespace {
 // neighbouring threads, each with 16 bytes of it a load, and a thread takes up
 // to kRows rows of one token with all their loads in flight before the first
 // use; the token's angles, sequence and page are looked up meanwhile, once.
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kRows = 4;
 
 struct AppendArgs {
@@ -53,34 +56,43 @@ struct AppendArgs {
   void* q_out;
 };
 
-// N consecutive elements as float32 and back, in accesses of up to 16 bytes.
+// N consecutive elements as loaded (4, 8 or a multiple of 16 bytes), as
+// float32, and back.
 template <typename T, int N>
-TL_DEV void load_n(const T* p, float* x) {
-  constexpr int B = N * sizeof(T);
+struct Raw {
+  static constexpr int B = N * sizeof(T);
   static_assert(B == 4 || B == 8 || B % 16 == 0, "whole accesses");
   uint32_t w[B / 4];
-  if constexpr (B == 4) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  } else if constexpr (B == 8) {
-    const uint2 y = *reinterpret_cast<const uint2*>(p);
-    w[0] = y.x, w[1] = y.y;
-  } else {
+  TL_DEV void load(const T* p) {
+    if constexpr (B == 4) {
+      w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (B == 8) {
+      const uint2 y = *reinterpret_cast<const uint2*>(p);
+      w[0] = y.x, w[1] = y.y;
+    } else {
 #pragma unroll
-    for (int i = 0; i < B / 16; ++i) {
-      const uint4 y = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) + 16 * i);
-      w[4 * i] = y.x, w[4 * i + 1] = y.y, w[4 * i + 2] = y.z, w[4 * i + 3] = y.w;
+      for (int i = 0; i < B / 16; ++i) {
+        const uint4 y = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(p) + 16 * i);
+        w[4 * i] = y.x, w[4 * i + 1] = y.y, w[4 * i + 2] = y.z, w[4 * i + 3] = y.w;
+      }
     }
   }
+  TL_DEV void clear() {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if constexpr (sizeof(T) == 4)
-      x[i] = __uint_as_float(w[i]);
-    else if constexpr (sizeof(T) == 2)
-      x[i] = to_f32(reinterpret_cast<const T*>(w)[i]);
-    else
-      x[i] = static_cast<float>(static_cast<int8_t>(w[i / 4] >> (8 * (i % 4))));
+    for (int i = 0; i < B / 4; ++i) w[i] = 0;
   }
-}
+  TL_DEV float operator[](int i) const {
+    if constexpr (sizeof(T) == 4)
+      return __uint_as_float(w[i]);
+    else if constexpr (sizeof(T) == 1)
+      return static_cast<float>(static_cast<int8_t>(w[i / 4] >> (8 * (i % 4))));
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+      return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else
+      return i % 2 ? __high2float(*reinterpret_cast<const __half2*>(w + i / 2))
+                   : __low2float(*reinterpret_cast<const __half2*>(w + i / 2));
+  }
+};
 template <typename T, int N>
 TL_DEV void store_n(T* p, const float* x) {
   constexpr int B = N * sizeof(T);
@@ -101,7 +113,7 @@ TL_DEV void store_n(T* p, const float* x) {
 // the reference's values), and quantize_int8 of the whole row, whose maximum
 // is taken over the row's threads. A thread holds N pairs, 16 bytes of each
 // half; D = 64, 32 + 2 * 4 head rows of bfloat16: 10 KB a token moved.
-// Measured: 16384 such tokens (171 MB) {T_PROMPT}, one token {T_ONE}.
+// Measured: 16721 such tokens (172 MB) 32.4 us, 5.3 TB/s; one token 2.2 us.
 template <typename TI, typename TC, int D>
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int N = 16 / sizeof(TI), LANES = D / 2 / N;  // pairs of a thread, threads of a row
@@ -113,7 +125,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
   const bool in = t < a.tokens;  // (the row maxima below are warp-wide)
   const int rows = a.heads + 2 * a.c.hkv;
 
-  float lo[kRows][N], hi[kRows][N];
+  const int p = in ? a.pos[t] : -1, s = in ? a.seq[t] : -1;  // the longest chain of loads starts here
+  Raw<TI, N> in_lo[kRows], in_hi[kRows];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const int r = g + u * a.groups;
@@ -122,15 +135,14 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
                   : r < a.heads + a.c.hkv
                       ? static_cast<const TI*>(a.k) + t * a.ldk + (r - a.heads) * D
                       : static_cast<const TI*>(a.v) + t * a.ldv + (r - a.heads - a.c.hkv) * D;
-    load_n<TI, N>(x + j, lo[u]);
-    load_n<TI, N>(x + j + D / 2, hi[u]);
+    in_lo[u].load(x + j);
+    in_hi[u].load(x + j + D / 2);
   }
-  const int p = in ? a.pos[t] : -1, s = in ? a.seq[t] : -1;
   const bool angle = !a.cos || (p >= 0 && p < a.max_pos);
-  float cs[N], sn[N];
+  Raw<float, N> cs, sn;
   if (a.cos && angle) {
-    load_n<float, N>(a.cos + static_cast<int64_t>(p) * D + j, cs);
-    load_n<float, N>(a.sin + static_cast<int64_t>(p) * D + j, sn);
+    cs.load(a.cos + static_cast<int64_t>(p) * D + j);
+    sn.load(a.sin + static_cast<int64_t>(p) * D + j);
   }
   const int64_t row0 = angle ? paged_row(a.c, s, p) : -1;
 
@@ -139,22 +151,28 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
     const int r = g + u * a.groups;
     const bool query = r < a.heads, key = !query && r < a.heads + a.c.hkv;
     const bool here = in && r < rows;
-    if (here && (query || key) && a.cos && angle) {
+    float lo[N], hi[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      lo[i] = here ? in_lo[u][i] : 0.0f;
+      hi[i] = here ? in_hi[u][i] : 0.0f;
+    }
+    if ((query || key) && a.cos && angle) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float x = lo[u][i], y = hi[u][i];
-        lo[u][i] = __fsub_rn(__fmul_rn(x, cs[i]), __fmul_rn(y, sn[i]));
-        hi[u][i] = __fadd_rn(__fmul_rn(y, cs[i]), __fmul_rn(x, sn[i]));
+        const float x = lo[i], y = hi[i];
+        lo[i] = __fsub_rn(__fmul_rn(x, cs[i]), __fmul_rn(y, sn[i]));
+        hi[i] = __fadd_rn(__fmul_rn(y, cs[i]), __fmul_rn(x, sn[i]));
       }
     }
     if (here && query) {
       TI* o = static_cast<TI*>(a.q_out) + (t * a.heads + r) * D + j;
       if (!angle) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) lo[u][i] = hi[u][i] = 0.0f;
+        for (int i = 0; i < N; ++i) lo[i] = hi[i] = 0.0f;
       }
-      store_n<TI, N>(o, lo[u]);
-      store_n<TI, N>(o + D / 2, hi[u]);
+      store_n<TI, N>(o, lo);
+      store_n<TI, N>(o + D / 2, hi);
     }
     const int64_t row = row0 + static_cast<int64_t>(r - a.heads - (key ? 0 : a.c.hkv)) * a.c.ps;
     TC* o = static_cast<TC*>(key ? a.c.k : a.c.v) + row * D + j;
@@ -165,10 +183,10 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
       float m = 0.0f;
       if (store) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) m = fmaxf(m, fmaxf(fabsf(lo[u][i]), fabsf(hi[u][i])));
+        for (int i = 0; i < N; ++i) m = fmaxf(m, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
 #pragma unroll
         for (int i = 0; i < N; ++i)
-          if (lo[u][i] != lo[u][i] || hi[u][i] != hi[u][i]) m = INFINITY;
+          if (lo[i] != lo[i] || hi[i] != hi[i]) m = INFINITY;
       }
 #pragma unroll
       for (int w = 1; w < LANES; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
@@ -185,8 +203,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
         if (!bad) {
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            x[i / 4] |= quantize(lo[u][i]) << (8 * (i % 4));
-            y[i / 4] |= quantize(hi[u][i]) << (8 * (i % 4));
+            x[i / 4] |= quantize(lo[i]) << (8 * (i % 4));
+            y[i / 4] |= quantize(hi[i]) << (8 * (i % 4));
           }
         }
         if constexpr (N == 4) {
@@ -199,14 +217,14 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
         if (j == 0) (key ? a.c.ks : a.c.vs)[row] = sc;
       }
     } else if (store) {
-      store_n<TC, N>(o, lo[u]);
-      store_n<TC, N>(o + D / 2, hi[u]);
+      store_n<TC, N>(o, lo);
+      store_n<TC, N>(o + D / 2, hi);
     }
   }
 }
 
 // Rows back as float32 or 16 bits: 16 bytes of output a thread and row.
-// Measured: 28791 tokens of 8 heads of 128 (bfloat16, 236 MB) {T_READ}.
+// Measured: 32593 tokens of 8 heads of 128 (bfloat16, 267 MB) 45.8 us, 5.8 TB/s.
 template <typename TC, typename TO, int D>
 __global__ void __launch_bounds__(kThreads)
     read_kernel(const __grid_constant__ PagedView c, const int32_t* seq, const int32_t* pos, int32_t tokens,
@@ -219,17 +237,17 @@ __global__ void __launch_bounds__(kThreads)
   const int g = static_cast<int>(part - static_cast<unsigned>(t) * groups);
   if (t >= tokens) return;
   const int64_t row0 = paged_row(c, seq[t], pos[t]);
-  float x[kRows][N], sc[kRows];
+  Raw<TC, N> x[kRows];
+  float sc[kRows];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const int r = g + u * groups;
     const bool key = r < c.hkv;
     const int64_t row = row0 + static_cast<int64_t>(key ? r : r - c.hkv) * c.ps;
     sc[u] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[u][i] = 0.0f;
+    x[u].clear();
     if (row0 < 0 || r >= 2 * c.hkv || !(key ? k_out : v_out)) continue;
-    load_n<TC, N>(static_cast<const TC*>(key ? c.k : c.v) + row * D + j, x[u]);
+    x[u].load(static_cast<const TC*>(key ? c.k : c.v) + row * D + j);
     if constexpr (sizeof(TC) == 1) sc[u] = (key ? c.ks : c.vs)[row];
   }
 #pragma unroll
@@ -237,17 +255,21 @@ __global__ void __launch_bounds__(kThreads)
     const int r = g + u * groups;
     TO* o = r < c.hkv ? k_out : v_out;
     if (r >= 2 * c.hkv || !o) continue;
-    if constexpr (sizeof(TC) == 1) {
+    float y[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[u][i] = __fmul_rn(x[u][i], sc[u]);
-    }
-    store_n<TO, N>(o + (t * c.hkv + (r < c.hkv ? r : r - c.hkv)) * D + j, x[u]);
+    for (int i = 0; i < N; ++i) y[i] = sizeof(TC) == 1 ? __fmul_rn(x[u][i], sc[u]) : x[u][i];
+    store_n<TO, N>(o + (t * c.hkv + (r < c.hkv ? r : r - c.hkv)) * D + j, y);
   }
 }
 
-// CTAs for `rows` rows of `lanes` threads a token; false if a grid cannot hold them.
+// Thread groups of a token and the grid for `rows` rows of `lanes` threads:
+// one row a thread while that leaves SMs idle (one token of 40 rows 2.2
+// against 2.4 us), then four, so that more of a token's bytes are in flight a
+// thread and its angles and page are looked up less often (16 prompts: see
+// above; with one row 40 us). False if the grid cannot hold them.
 bool grid_for(int tokens, int rows, int lanes, int* groups, unsigned* grid) {
-  *groups = (rows + kRows - 1) / kRows;
+  const int64_t threads = static_cast<int64_t>(tokens) * rows * lanes;
+  *groups = threads <= static_cast<int64_t>(device_sm_count()) * 1024 ? rows : (rows + kRows - 1) / kRows;
   const int64_t ctas = (static_cast<int64_t>(tokens) * *groups * lanes + kThreads - 1) / kThreads;
   *grid = static_cast<unsigned>(ctas);
   return static_cast<int64_t>(tokens) * *groups + kThreads <= INT32_MAX && ctas <= INT32_MAX;
