@@ -32,9 +32,14 @@ class PagedView(C.Structure):
                 ("head_dim", C.c_int32)]
 
 
-def _torch():
-    import torch
-    if not _FLOAT_CODES:
+torch = None  # imported by the first call that needs it (importing the package does not)
+
+
+def _need_torch():
+    global torch
+    if torch is None:
+        import torch as module
+        torch = module
         _FLOAT_CODES.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
         _POOL_CODES.update({torch.int8: I8, torch.bfloat16: BF16, torch.float16: F16})
     return torch
@@ -47,36 +52,44 @@ def _bad(name, t, want):
 
 def _index(name, t, n, dev):
     """int32 vector of n entries on the device -> its address."""
-    torch = _torch()
-    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.shape == (n,) and t.device == dev
-            and (n < 2 or t.stride(0) == 1)):
-        raise _bad(name, t, f"a contiguous int32 [{n}] tensor on {dev}")
-    return t.data_ptr()
+    if (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == (n,) and t.device == dev
+            and t.is_contiguous()):
+        return t.data_ptr()
+    raise _bad(name, t, f"a contiguous int32 [{n}] tensor on {dev}")
 
 
 def _rows(name, t, n, heads, d, dtype, dev):
     """[n, heads, d] activations with contiguous head rows, 16-byte aligned -> (address, row stride)."""
-    torch = _torch()
-    if isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == (n, heads, d) and t.device == dev:
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (n, heads, d) and t.device == dev:
         s0, s1, s2 = t.stride()
         p = t.data_ptr()
         if n < 2:
             s0 = heads * d
-        if s2 == 1 and (s1 == d or heads == 1) and s0 >= heads * d and not (p | s0 * t.element_size()) & 15:
+        if s2 == 1 and (s1 == d or heads == 1) and s0 >= heads * d and not (p | s0 * dtype.itemsize) & 15:
             return p, s0
     raise _bad(name, t, f"a {dtype} [{n}, {heads}, {d}] tensor on {dev}, head rows contiguous, tokens a multiple of "
                         "16 bytes apart, 16-byte aligned")
 
 
-def _out(name, t, shape, dtype, dev):
-    """``t`` checked as a contiguous output, or a new tensor."""
-    torch = _torch()
+def _out(name, t, like, shape, dtype):
+    """``t`` checked as a contiguous output on ``like``'s device, or a new tensor."""
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=dev)
-    if not (isinstance(t, torch.Tensor) and t.dtype == dtype and t.shape == shape and t.device == dev
+        return like.new_empty(shape, dtype=dtype)
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == like.device
             and t.is_contiguous() and not t.data_ptr() & 15):
-        raise _bad(name, t, f"a contiguous {dtype} {list(shape)} tensor on {dev}, 16-byte aligned")
+        raise _bad(name, t, f"a contiguous {dtype} {list(shape)} tensor on {like.device}, 16-byte aligned")
     return t
+
+
+def _enqueue(what, fn, index, *args):
+    """Calls a library entry on the current stream of device ``index``, with that device current."""
+    if torch.cuda.current_device() == index:
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        check(code, what)
 
 
 class PagedKVCache:
@@ -99,7 +112,7 @@ class PagedKVCache:
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=None, device="cuda"):
         """Allocates the pool, zeroed; ``dtype`` is torch.int8 (default), bfloat16 or float16."""
-        torch = _torch()
+        _need_torch()
         dtype = torch.int8 if dtype is None else dtype
         if dtype not in _POOL_CODES:
             raise ValueError(f"dtype must be one of {[str(x) for x in _POOL_CODES]}, got {dtype}")
@@ -121,7 +134,7 @@ class PagedKVCache:
         return self
 
     def _bind(self, k, v, k_scale, v_scale):
-        torch = _torch()
+        _need_torch()
         for name, t in (("k", k), ("v", v)):
             if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 4 and t.dtype in _POOL_CODES
                     and t.numel() and t.is_contiguous() and not t.data_ptr() & 15):
@@ -141,7 +154,9 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.dtype, self.device = k.dtype, k.device
-        self._lib = load_library()
+        self._index = k.device.index
+        self._lib = lib = load_library()
+        self._append, self._read, self._attend = lib.tl_paged_append, lib.tl_paged_read, lib.tl_paged_attn_decode
         ptr = [t.data_ptr() if t is not None else None for t in (k, v, k_scale, v_scale)]
         self._view = PagedView(*ptr, _POOL_CODES[k.dtype], *k.shape)
         self._ref = C.byref(self._view)
@@ -150,26 +165,16 @@ class PagedKVCache:
         self._work_bytes = 0
 
     # ---------------------------------------------------------------- calls
-    def _call(self, name, *args):
-        torch = _torch()
-        if torch.cuda.current_device() == self.device.index:
-            code = getattr(self._lib, name)(*args, torch.cuda.current_stream().cuda_stream)
-        else:
-            with torch.cuda.device(self.device):
-                code = getattr(self._lib, name)(*args, torch.cuda.current_stream().cuda_stream)
-        if code:
-            check(code, name)
-
     def _table(self, t):
-        torch = _torch()
-        if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.dim() == 2 and t.device == self.device
-                and t.shape[0] and t.shape[1] and (t.shape[1] == 1 or t.stride(1) == 1)):
-            raise _bad("block_table", t, f"an int32 [n_seqs, max_pages] tensor on {self.device} with contiguous rows")
-        n, m = t.shape
-        stride = t.stride(0) if n > 1 else m
-        if stride < m:
-            raise _bad("block_table", t, "a table whose rows do not overlap")
-        return t.data_ptr(), n, m, stride
+        if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 2 and t.device == self.device:
+            n, m = t.shape
+            stride, one = t.stride()
+            if n < 2:
+                stride = m
+            if n and m and (one == 1 or m == 1) and stride >= m:
+                return t.data_ptr(), n, m, stride
+        raise _bad("block_table", t, f"an int32 [n_seqs, max_pages] tensor on {self.device} with contiguous rows that "
+                                     "do not overlap")
 
     def append(self, k, v, block_table, seq, pos, cos=None, sin=None, q=None, q_out=None):
         """Stores key and value rows ``k``, ``v`` ``[tokens, kv_heads, head_dim]`` at
@@ -185,7 +190,6 @@ class PagedKVCache:
         that name no row store nothing; a position beyond the angles stores
         nothing and gives a zero query row.
         """
-        torch = _torch()
         if not isinstance(k, torch.Tensor) or k.dim() != 3 or k.dtype not in _FLOAT_CODES:
             raise _bad("k", k, "a float32, bfloat16 or float16 [tokens, kv_heads, head_dim] tensor")
         n, dt, dev, d = k.shape[0], k.dtype, self.device, self.head_dim
@@ -195,14 +199,14 @@ class PagedKVCache:
         sp, pp = _index("seq", seq, n, dev), _index("pos", pos, n, dev)
         if (cos is None) != (sin is None):
             raise ValueError("cos and sin go together")
-        cp = np_ = n_ang = None
+        cosp, sinp, n_ang = None, None, 0
         if cos is not None:
             for name, t in (("cos", cos), ("sin", sin)):
-                if not (isinstance(t, torch.Tensor) and t.dtype == torch.float32 and t.dim() == 2 and t.shape[0]
-                        and t.shape[1] == d and t.shape == cos.shape and t.device == dev and t.is_contiguous()
+                if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.dim() == 2 and t.shape[1] == d
+                        and t.shape == cos.shape and t.shape[0] and t.device == dev and t.is_contiguous()
                         and not t.data_ptr() & 15):
                     raise _bad(name, t, f"a contiguous float32 [max_positions, {d}] tensor on {dev}")
-            cp, np_, n_ang = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
+            cosp, sinp, n_ang = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
         qp, qs, heads, op = None, 0, 0, None
         if q is not None:
             if cos is None:
@@ -211,20 +215,19 @@ class PagedKVCache:
                 raise _bad("q", q, "a [tokens, heads, head_dim] tensor")
             heads = q.shape[1]
             qp, qs = _rows("q", q, n, heads, d, dt, dev)
-            q_out = _out("q_out", q_out, (n, heads, d), dt, dev)
+            q_out = _out("q_out", q_out, q, (n, heads, d), dt)
             op = q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
         if n:
-            self._call("tl_paged_append", self._ref, qp, kp, vp, _FLOAT_CODES[dt], qs, ks, vs, sp, pp, *tab, cp, np_,
-                       n_ang or 0, n, heads, op)
+            _enqueue("tl_paged_append", self._append, self._index, self._ref, qp, kp, vp, _FLOAT_CODES[dt], qs, ks, vs,
+                     sp, pp, *tab, cosp, sinp, n_ang, n, heads, op)
         return q_out
 
     def read(self, block_table, seq, pos, dtype=None, k_out=None, v_out=None):
         """Rows ``(seq[t], pos[t])`` as ``(k, v)``, each ``[tokens, kv_heads, head_dim]`` of
         ``dtype`` (float32 by default; tl_paged_read). Keys are as stored, rotated.
         Tokens that name no row give zeros."""
-        torch = _torch()
         dtype = torch.float32 if dtype is None else dtype
         if dtype not in _FLOAT_CODES:
             raise ValueError(f"dtype must be one of {[str(x) for x in _FLOAT_CODES]}, got {dtype}")
@@ -234,9 +237,10 @@ class PagedKVCache:
         tab = self._table(block_table)
         sp, pp = _index("seq", seq, n, dev), _index("pos", pos, n, dev)
         shape = (n, self.kv_heads, self.head_dim)
-        k, v = _out("k_out", k_out, shape, dtype, dev), _out("v_out", v_out, shape, dtype, dev)
+        k, v = _out("k_out", k_out, self.k, shape, dtype), _out("v_out", v_out, self.k, shape, dtype)
         if n:
-            self._call("tl_paged_read", self._ref, sp, pp, *tab, n, k.data_ptr(), v.data_ptr(), _FLOAT_CODES[dtype])
+            _enqueue("tl_paged_read", self._read, self._index, self._ref, sp, pp, *tab, n, k.data_ptr(), v.data_ptr(),
+                     _FLOAT_CODES[dtype])
         return k, v
 
     def attend(self, q, block_table, lengths, seq=None, sm_scale=None, out=None, return_lse=False, lse=None):
@@ -251,7 +255,6 @@ class PagedKVCache:
         ``[rows, heads]`` of the scores. A row without positions gives zeros and
         -inf.
         """
-        torch = _torch()
         if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _FLOAT_CODES:
             raise _bad("q", q, "a float32, bfloat16 or float16 [rows, heads, head_dim] tensor")
         n, heads, d = q.shape
@@ -268,14 +271,14 @@ class PagedKVCache:
             raise ValueError(f"{n} rows but the table has {tab[1]} sequences: pass seq")
         else:
             sp = None
-        out = _out("out", out, (n, heads, d), dt, dev)
+        out = _out("out", out, q, (n, heads, d), dt)
         if return_lse or lse is not None:
-            lse = _out("lse", lse, (n, heads), torch.float32, dev)
+            lse = _out("lse", lse, q, (n, heads), torch.float32)
         if n:
             work = self._workspace(heads)
-            self._call("tl_paged_attn_decode", self._ref, qp, _FLOAT_CODES[dt], qs, sp, lp, *tab, n, heads,
-                       self._scale if sm_scale is None else float(sm_scale), out.data_ptr(),
-                       lse.data_ptr() if lse is not None else None, work, self._work_bytes)
+            _enqueue("tl_paged_attn_decode", self._attend, self._index, self._ref, qp, _FLOAT_CODES[dt], qs, sp, lp,
+                     *tab, n, heads, self._scale if sm_scale is None else float(sm_scale), out.data_ptr(),
+                     lse.data_ptr() if lse is not None else None, work, self._work_bytes)
         return (out, lse) if return_lse else out
 
     def _workspace(self, heads):
@@ -283,7 +286,6 @@ class PagedKVCache:
         (make that call before capturing a graph) and kept: its size does not
         depend on rows or lengths."""
         if self._work is None or self._work[1] < heads:
-            torch = _torch()
             need = self._lib.tl_paged_attn_workspace_bytes(heads, self.kv_heads, self.head_dim)
             kept = self._work  # a larger one may follow while calls that use this one are in flight
             if need > self._work_bytes:
@@ -309,7 +311,7 @@ def token_logprobs(logits, tokens=None, top_k: int = 0) -> TokenLogprobs:
     id. Logits of -inf have probability 0 and are never listed (id -1, -inf).
     A negative token gives 0, one beyond the vocabulary NaN; a row with a NaN or
     +inf gives NaN everywhere."""
-    torch = _torch()
+    _need_torch()
     if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dim() == 2 and logits.dtype in _FLOAT_CODES
             and logits.shape[1] and (logits.shape[1] == 1 or logits.stride(1) == 1)):
         raise _bad("logits", logits, "a CUDA tensor [rows, vocab] of float32, bfloat16 or float16 with contiguous rows")
@@ -322,16 +324,16 @@ def token_logprobs(logits, tokens=None, top_k: int = 0) -> TokenLogprobs:
         raise ValueError(f"top_k must be in 0..{TOP_K_MAX}, got {top_k}")
     tp = _index("tokens", tokens, n, dev) if tokens is not None else None
     f32 = torch.float32
-    lp = torch.empty(n, dtype=f32, device=dev) if tokens is not None else None
-    ent = torch.empty(n, dtype=f32, device=dev)
-    ids = torch.empty((n, top_k), dtype=torch.int32, device=dev)
-    top = torch.empty((n, top_k), dtype=f32, device=dev)
+    # the float32 results share one allocation
+    if tokens is None:
+        lp = None
+        ent, top = logits.new_empty(n * (1 + top_k), dtype=f32).split_with_sizes((n, n * top_k))
+    else:
+        lp, ent, top = logits.new_empty(n * (2 + top_k), dtype=f32).split_with_sizes((n, n, n * top_k))
+    top = top.view(n, top_k)
+    ids = logits.new_empty((n, top_k), dtype=torch.int32)
     if n:
-        with torch.cuda.device(dev):
-            code = load_library().tl_token_logprobs(
-                logits.data_ptr(), _FLOAT_CODES[logits.dtype], stride, tp, n, vocab, top_k,
-                lp.data_ptr() if lp is not None else None, ent.data_ptr(), ids.data_ptr() if top_k else None,
-                top.data_ptr() if top_k else None, torch.cuda.current_stream().cuda_stream)
-        if code:
-            check(code, "tl_token_logprobs")
+        _enqueue("tl_token_logprobs", load_library().tl_token_logprobs, dev.index, logits.data_ptr(),
+                 _FLOAT_CODES[logits.dtype], stride, tp, n, vocab, top_k, lp.data_ptr() if lp is not None else None,
+                 ent.data_ptr(), ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None)
     return TokenLogprobs(lp, ent, ids, top)
