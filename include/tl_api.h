@@ -565,18 +565,45 @@ typedef struct tl_paged_kv {
  * NULL stores keys as they are (q must be NULL): rows that tl_paged_read gave
  * from another pool. Two tokens of a call must not name one row. A row with an
  * infinity or a NaN gets a NaN scale in a TL_I8 pool. */
-TL_API tl_status tl_paged_append(const tl_paged_kv* cache, const void* q, const void* k, const void* v, int32_t dtype,
-                                 int64_t q_stride, int64_t k_stride, int64_t v_stride, const int32_t* seq,
-                                 const int32_t* pos, const int32_t* block_table, int32_t n_seqs, int32_t max_pages,
-                                 int64_t table_stride, const float* rope_cos, const float* rope_sin,
-                                 int32_t max_positions, int32_t tokens, int32_t heads, void* q_out, void* stream);
+typedef struct tl_paged_append_args {
+  const void* q;            /* NULL: no queries */
+  const void* k;
+  const void* v;
+  void* q_out;
+  const int32_t* seq;       /* [tokens] */
+  const int32_t* pos;       /* [tokens] */
+  const int32_t* block_table;
+  const float* rope_cos;    /* [max_positions][head_dim], both NULL: no rotation */
+  const float* rope_sin;
+  int64_t q_stride;         /* elements between tokens */
+  int64_t k_stride;
+  int64_t v_stride;
+  int64_t table_stride;
+  int32_t dtype;            /* of q, k, v and q_out */
+  int32_t n_seqs;
+  int32_t max_pages;
+  int32_t max_positions;
+  int32_t tokens;
+  int32_t heads;            /* query heads */
+} tl_paged_append_args;
+TL_API tl_status tl_paged_append(const tl_paged_kv* cache, const tl_paged_append_args* args, void* stream);
 
 /* Reads rows (seq[t], pos[t]) back into k_out, v_out [tokens][kv_heads][head_dim]
  * of out_dtype (TL_F32, TL_BF16 or TL_F16), contiguous, 16-byte aligned,
  * rounded once; either may be NULL. Tokens that name no row give zeros. */
-TL_API tl_status tl_paged_read(const tl_paged_kv* cache, const int32_t* seq, const int32_t* pos,
-                               const int32_t* block_table, int32_t n_seqs, int32_t max_pages, int64_t table_stride,
-                               int32_t tokens, void* k_out, void* v_out, int32_t out_dtype, void* stream);
+typedef struct tl_paged_read_args {
+  const int32_t* seq;       /* [tokens] */
+  const int32_t* pos;       /* [tokens] */
+  const int32_t* block_table;
+  void* k_out;
+  void* v_out;
+  int64_t table_stride;
+  int32_t n_seqs;
+  int32_t max_pages;
+  int32_t tokens;
+  int32_t out_dtype;
+} tl_paged_read_args;
+TL_API tl_status tl_paged_read(const tl_paged_kv* cache, const tl_paged_read_args* args, void* stream);
 
 /* Attention of one new token of each of `rows` sequences over the pool: for
  * row r and query head h (kv head h / (heads / kv_heads)) over positions
@@ -596,11 +623,25 @@ TL_API tl_status tl_paged_read(const tl_paged_kv* cache, const int32_t* seq, con
  * next. Calls that share one workspace must not overlap on the GPU. The call
  * allocates nothing, does not synchronise and can be captured in a graph. */
 TL_API size_t tl_paged_attn_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t head_dim);
-TL_API tl_status tl_paged_attn_decode(const tl_paged_kv* cache, const void* q, int32_t q_dtype, int64_t q_stride,
-                                      const int32_t* seq, const int32_t* lengths, const int32_t* block_table,
-                                      int32_t n_seqs, int32_t max_pages, int64_t table_stride, int32_t rows,
-                                      int32_t heads, float sm_scale, void* out, float* lse, void* workspace,
-                                      size_t workspace_bytes, void* stream);
+typedef struct tl_paged_attn_args {
+  const void* q;
+  const int32_t* seq;       /* [rows], NULL: sequence r */
+  const int32_t* lengths;   /* [rows] */
+  const int32_t* block_table;
+  void* out;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t q_stride;         /* elements between rows */
+  int64_t table_stride;
+  int32_t q_dtype;
+  int32_t n_seqs;
+  int32_t max_pages;
+  int32_t rows;
+  int32_t heads;
+  float sm_scale;
+} tl_paged_attn_args;
+TL_API tl_status tl_paged_attn_decode(const tl_paged_kv* cache, const tl_paged_attn_args* args, void* stream);
 
 /* Log probabilities of given tokens, entropy and the top_k most likely tokens
  * of each row of logits [rows][vocab] (TL_F32, TL_BF16 or TL_F16; rows
@@ -616,9 +657,20 @@ TL_API tl_status tl_paged_attn_decode(const tl_paged_kv* cache, const void* q, i
  * row with a NaN or +infinity has no distribution: logprob, entropy and
  * top_logprobs are NaN, ids -1. Needs no workspace. */
 #define TL_TOP_K_MAX 32
-TL_API tl_status tl_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, const int32_t* tokens,
-                                   int32_t rows, int32_t vocab, int32_t top_k, float* logprob, float* entropy,
-                                   int32_t* top_ids, float* top_logprobs, void* stream);
+typedef struct tl_token_logprobs_args {
+  const void* logits;
+  const int32_t* tokens;    /* [rows], NULL: logprob is not written */
+  float* logprob;           /* [rows] */
+  float* entropy;           /* [rows] */
+  int32_t* top_ids;         /* [rows][top_k] */
+  float* top_logprobs;      /* [rows][top_k] */
+  int64_t row_stride;
+  int32_t dtype;
+  int32_t rows;
+  int32_t vocab;
+  int32_t top_k;
+} tl_token_logprobs_args;
+TL_API tl_status tl_token_logprobs(const tl_token_logprobs_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -425,17 +425,19 @@ tl_status logprob_launch(const LogprobArgs& a, cudaStream_t s) {
 
 using namespace tl;
 
-extern "C" tl_status tl_token_logprobs(const void* logits, int32_t dtype, int64_t row_stride, const int32_t* tokens,
-                                       int32_t rows, int32_t vocab, int32_t top_k, float* logprob, float* entropy,
-                                       int32_t* top_ids, float* top_logprobs, void* stream) {
-  if (!logits || !is_float_dtype(dtype) || rows <= 0 || vocab <= 0 || row_stride < vocab) return TL_ERR_INVALID_ARGUMENT;
-  if (!aligned_to(logits, dtype_bytes(dtype)) || !tokens != !logprob) return TL_ERR_INVALID_ARGUMENT;
-  if (top_k < 0 || (top_k > 0 && (!top_ids || !top_logprobs))) return TL_ERR_INVALID_ARGUMENT;
-  if (!logprob && !entropy && !top_k) return TL_ERR_INVALID_ARGUMENT;
-  if (top_k > TL_TOP_K_MAX) return TL_ERR_OUT_OF_RANGE;
-  const LogprobArgs a{logits, row_stride, tokens, rows, vocab, top_k, logprob, entropy, top_logprobs, top_ids};
+extern "C" tl_status tl_token_logprobs(const tl_token_logprobs_args* args, void* stream) {
+  if (!args) return TL_ERR_INVALID_ARGUMENT;
+  const tl_token_logprobs_args& x = *args;
+  if (!x.logits || !is_float_dtype(x.dtype) || x.rows <= 0 || x.vocab <= 0 || x.row_stride < x.vocab)
+    return TL_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(x.logits, dtype_bytes(x.dtype)) || !x.tokens != !x.logprob) return TL_ERR_INVALID_ARGUMENT;
+  if (x.top_k < 0 || (x.top_k > 0 && (!x.top_ids || !x.top_logprobs))) return TL_ERR_INVALID_ARGUMENT;
+  if (!x.logprob && !x.entropy && !x.top_k) return TL_ERR_INVALID_ARGUMENT;
+  if (x.top_k > TL_TOP_K_MAX) return TL_ERR_OUT_OF_RANGE;
+  const LogprobArgs a{x.logits, x.row_stride, x.tokens,  x.rows,         x.vocab,
+                      x.top_k,  x.logprob,    x.entropy, x.top_logprobs, x.top_ids};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == TL_F32    ? logprob_launch<float>(a, s)
-         : dtype == TL_BF16 ? logprob_launch<__nv_bfloat16>(a, s)
-                            : logprob_launch<__half>(a, s);
+  return x.dtype == TL_F32    ? logprob_launch<float>(a, s)
+         : x.dtype == TL_BF16 ? logprob_launch<__nv_bfloat16>(a, s)
+                              : logprob_launch<__half>(a, s);
 }

@@ -326,62 +326,61 @@ using namespace tl;
 
 extern "C" {
 
-tl_status tl_paged_append(const tl_paged_kv* cache, const void* q, const void* k, const void* v, int32_t dtype,
-                          int64_t q_stride, int64_t k_stride, int64_t v_stride, const int32_t* seq,
-                          const int32_t* pos, const int32_t* block_table, int32_t n_seqs, int32_t max_pages,
-                          int64_t table_stride, const float* rope_cos, const float* rope_sin, int32_t max_positions,
-                          int32_t tokens, int32_t heads, void* q_out, void* stream) {
+tl_status tl_paged_append(const tl_paged_kv* cache, const tl_paged_append_args* args, void* stream) {
+  if (!cache || !args) return TL_ERR_INVALID_ARGUMENT;
+  const tl_paged_append_args& x = *args;
   AppendArgs a;
-  const tl_status st = paged_view(cache, block_table, n_seqs, max_pages, table_stride, &a.c);
+  const tl_status st = paged_view(cache, x.block_table, x.n_seqs, x.max_pages, x.table_stride, &a.c);
   if (st != TL_OK) return st;
-  if (!k || !v || !seq || !pos || !is_float_dtype(dtype) || tokens <= 0) return TL_ERR_INVALID_ARGUMENT;
-  if (!rope_cos != !rope_sin || (rope_cos && max_positions <= 0)) return TL_ERR_INVALID_ARGUMENT;
-  if (!q != !q_out || (q && (heads <= 0 || !rope_cos))) return TL_ERR_INVALID_ARGUMENT;
-  const int64_t d = cache->head_dim, e = dtype_bytes(dtype), kv = cache->kv_heads;
-  if (k_stride < kv * d || v_stride < kv * d || (q && q_stride < heads * d)) return TL_ERR_INVALID_ARGUMENT;
-  if (!aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(q, 16) || !aligned_to(q_out, 16) ||
-      (k_stride * e) % 16 || (v_stride * e) % 16 || (q && (q_stride * e) % 16) || !aligned_to(rope_cos, 16) ||
-      !aligned_to(rope_sin, 16))
+  if (!x.k || !x.v || !x.seq || !x.pos || !is_float_dtype(x.dtype) || x.tokens <= 0) return TL_ERR_INVALID_ARGUMENT;
+  if (!x.rope_cos != !x.rope_sin || (x.rope_cos && x.max_positions <= 0)) return TL_ERR_INVALID_ARGUMENT;
+  if (!x.q != !x.q_out || (x.q && (x.heads <= 0 || !x.rope_cos))) return TL_ERR_INVALID_ARGUMENT;
+  const int64_t d = cache->head_dim, e = dtype_bytes(x.dtype), kv = cache->kv_heads;
+  if (x.k_stride < kv * d || x.v_stride < kv * d || (x.q && x.q_stride < x.heads * d)) return TL_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(x.k, 16) || !aligned_to(x.v, 16) || !aligned_to(x.q, 16) || !aligned_to(x.q_out, 16) ||
+      (x.k_stride * e) % 16 || (x.v_stride * e) % 16 || (x.q && (x.q_stride * e) % 16) || !aligned_to(x.rope_cos, 16) ||
+      !aligned_to(x.rope_sin, 16))
     return TL_ERR_INVALID_ARGUMENT;
-  if (q == q_out && q && q_stride != heads * d) return TL_ERR_INVALID_ARGUMENT;
-  a.q = q;
-  a.k = k;
-  a.v = v;
-  a.ldq = q_stride;
-  a.ldk = k_stride;
-  a.ldv = v_stride;
-  a.seq = seq;
-  a.pos = pos;
-  a.cos = rope_cos;
-  a.sin = rope_sin;
-  a.max_pos = max_positions;
-  a.tokens = tokens;
-  a.heads = q ? heads : 0;
-  a.q_out = q_out;
+  if (x.q && x.q == x.q_out && x.q_stride != x.heads * d) return TL_ERR_INVALID_ARGUMENT;
+  a.q = x.q;
+  a.k = x.k;
+  a.v = x.v;
+  a.ldq = x.q_stride;
+  a.ldk = x.k_stride;
+  a.ldv = x.v_stride;
+  a.seq = x.seq;
+  a.pos = x.pos;
+  a.cos = x.rope_cos;
+  a.sin = x.rope_sin;
+  a.max_pos = x.max_positions;
+  a.tokens = x.tokens;
+  a.heads = x.q ? x.heads : 0;
+  a.q_out = x.q_out;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == TL_F32    ? append_pool<float>(a, cache->dtype, cache->head_dim, s)
-         : dtype == TL_BF16 ? append_pool<__nv_bfloat16>(a, cache->dtype, cache->head_dim, s)
-                            : append_pool<__half>(a, cache->dtype, cache->head_dim, s);
+  return x.dtype == TL_F32    ? append_pool<float>(a, cache->dtype, cache->head_dim, s)
+         : x.dtype == TL_BF16 ? append_pool<__nv_bfloat16>(a, cache->dtype, cache->head_dim, s)
+                              : append_pool<__half>(a, cache->dtype, cache->head_dim, s);
 }
 
-tl_status tl_paged_read(const tl_paged_kv* cache, const int32_t* seq, const int32_t* pos, const int32_t* block_table,
-                        int32_t n_seqs, int32_t max_pages, int64_t table_stride, int32_t tokens, void* k_out,
-                        void* v_out, int32_t out_dtype, void* stream) {
+tl_status tl_paged_read(const tl_paged_kv* cache, const tl_paged_read_args* args, void* stream) {
+  if (!cache || !args) return TL_ERR_INVALID_ARGUMENT;
+  const tl_paged_read_args& x = *args;
   ReadArgs a;
-  const tl_status st = paged_view(cache, block_table, n_seqs, max_pages, table_stride, &a.c);
+  const tl_status st = paged_view(cache, x.block_table, x.n_seqs, x.max_pages, x.table_stride, &a.c);
   if (st != TL_OK) return st;
-  if (!seq || !pos || tokens <= 0 || !is_float_dtype(out_dtype) || (!k_out && !v_out)) return TL_ERR_INVALID_ARGUMENT;
-  if (!aligned_to(k_out, 16) || !aligned_to(v_out, 16)) return TL_ERR_INVALID_ARGUMENT;
-  a.seq = seq;
-  a.pos = pos;
-  a.tokens = tokens;
-  a.k = k_out;
-  a.v = v_out;
+  if (!x.seq || !x.pos || x.tokens <= 0 || !is_float_dtype(x.out_dtype) || (!x.k_out && !x.v_out))
+    return TL_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(x.k_out, 16) || !aligned_to(x.v_out, 16)) return TL_ERR_INVALID_ARGUMENT;
+  a.seq = x.seq;
+  a.pos = x.pos;
+  a.tokens = x.tokens;
+  a.k = x.k_out;
+  a.v = x.v_out;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int d = cache->head_dim;
-  return cache->dtype == TL_I8     ? read_out<int8_t>(a, out_dtype, d, s)
-         : cache->dtype == TL_BF16 ? read_out<__nv_bfloat16>(a, out_dtype, d, s)
-                                   : read_out<__half>(a, out_dtype, d, s);
+  return cache->dtype == TL_I8     ? read_out<int8_t>(a, x.out_dtype, d, s)
+         : cache->dtype == TL_BF16 ? read_out<__nv_bfloat16>(a, x.out_dtype, d, s)
+                                   : read_out<__half>(a, x.out_dtype, d, s);
 }
 
 }  // extern "C"

@@ -969,35 +969,34 @@ size_t tl_paged_attn_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t he
   return kTicketBytes + static_cast<size_t>(kMaxCtas) * 2 * tile * (head_dim + 2) * sizeof(float);
 }
 
-tl_status tl_paged_attn_decode(const tl_paged_kv* cache, const void* q, int32_t q_dtype, int64_t q_stride,
-                               const int32_t* seq, const int32_t* lengths, const int32_t* block_table, int32_t n_seqs,
-                               int32_t max_pages, int64_t table_stride, int32_t rows, int32_t heads, float sm_scale,
-                               void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+tl_status tl_paged_attn_decode(const tl_paged_kv* cache, const tl_paged_attn_args* args, void* stream) {
+  if (!cache || !args) return TL_ERR_INVALID_ARGUMENT;
+  const tl_paged_attn_args& x = *args;
   AttendArgs a;
-  const tl_status st = paged_view(cache, block_table, n_seqs, max_pages, table_stride, &a.c);
+  const tl_status st = paged_view(cache, x.block_table, x.n_seqs, x.max_pages, x.table_stride, &a.c);
   if (st != TL_OK) return st;
-  if (!q || !lengths || !out || !workspace || !is_float_dtype(q_dtype) || rows <= 0 || heads <= 0)
+  if (!x.q || !x.lengths || !x.out || !x.workspace || !is_float_dtype(x.q_dtype) || x.rows <= 0 || x.heads <= 0)
     return TL_ERR_INVALID_ARGUMENT;
   const int64_t d = cache->head_dim;
-  if (heads % cache->kv_heads || q_stride < heads * d || (q_stride * dtype_bytes(q_dtype)) % 16)
+  if (x.heads % cache->kv_heads || x.q_stride < x.heads * d || (x.q_stride * dtype_bytes(x.q_dtype)) % 16)
     return TL_ERR_INVALID_ARGUMENT;
-  if (!aligned_to(q, 16) || !aligned_to(out, 16) || !aligned_to(workspace, 16)) return TL_ERR_INVALID_ARGUMENT;
-  if (workspace_bytes < tl_paged_attn_workspace_bytes(heads, cache->kv_heads, cache->head_dim))
+  if (!aligned_to(x.q, 16) || !aligned_to(x.out, 16) || !aligned_to(x.workspace, 16)) return TL_ERR_INVALID_ARGUMENT;
+  if (x.workspace_bytes < tl_paged_attn_workspace_bytes(x.heads, cache->kv_heads, cache->head_dim))
     return TL_ERR_OUT_OF_RANGE;
-  if (!seq && rows > n_seqs) return TL_ERR_OUT_OF_RANGE;
-  a.q = q;
-  a.ldq = q_stride;
-  a.q_dtype = q_dtype;
-  a.seq = seq;
-  a.lengths = lengths;
-  a.rows = rows;
-  a.heads = heads;
-  a.group = heads / cache->kv_heads;
-  a.scale = sm_scale;
-  a.out = out;
-  a.lse = lse;
-  a.tickets = static_cast<unsigned int*>(workspace);
-  a.records = reinterpret_cast<float*>(static_cast<char*>(workspace) + kTicketBytes);
+  if (!x.seq && x.rows > x.n_seqs) return TL_ERR_OUT_OF_RANGE;
+  a.q = x.q;
+  a.ldq = x.q_stride;
+  a.q_dtype = x.q_dtype;
+  a.seq = x.seq;
+  a.lengths = x.lengths;
+  a.rows = x.rows;
+  a.heads = x.heads;
+  a.group = x.heads / cache->kv_heads;
+  a.scale = x.sm_scale;
+  a.out = x.out;
+  a.lse = x.lse;
+  a.tickets = static_cast<unsigned int*>(x.workspace);
+  a.records = reinterpret_cast<float*>(static_cast<char*>(x.workspace) + kTicketBytes);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return cache->dtype == TL_I8     ? attend_dim<TL_I8>(a, cache->head_dim, s)
          : cache->dtype == TL_BF16 ? attend_dim<TL_BF16>(a, cache->head_dim, s)

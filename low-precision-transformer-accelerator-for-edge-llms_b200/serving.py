@@ -13,6 +13,7 @@ is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
+from struct import Struct
 from typing import NamedTuple
 
 from .shim import check, load_library
@@ -32,6 +33,12 @@ class PagedView(C.Structure):
                 ("head_dim", C.c_int32)]
 
 
+# tl_paged_append_args, tl_paged_read_args, tl_paged_attn_args, tl_token_logprobs_args
+_APPEND = Struct("@9P4q6i")
+_READ = Struct("@5Pq4i")
+_ATTEND = Struct("@7PN2q5if")
+_LOGPROBS = Struct("@6Pq4i")
+
 torch = None  # imported by the first call that needs it (importing the package does not)
 
 
@@ -50,25 +57,34 @@ def _bad(name, t, want):
     return ValueError(f"{name} must be {want}, got {got}")
 
 
-def _index(name, t, n, dev):
-    """int32 vector of n entries on the device -> its address."""
-    if (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == (n,) and t.device == dev
+def _index(name, t, n, gpu):
+    """int32 vector of n entries on device ``gpu`` -> its address."""
+    if (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == (n,) and t.get_device() == gpu
             and t.is_contiguous()):
         return t.data_ptr()
-    raise _bad(name, t, f"a contiguous int32 [{n}] tensor on {dev}")
+    raise _bad(name, t, f"a contiguous int32 [{n}] tensor on cuda:{gpu}")
 
 
-def _rows(name, t, n, heads, d, dtype, dev):
+def _rows(name, t, n, heads, d, dtype, gpu):
     """[n, heads, d] activations with contiguous head rows, 16-byte aligned -> (address, row stride)."""
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (n, heads, d) and t.device == dev:
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (n, heads, d) and t.get_device() == gpu:
         s0, s1, s2 = t.stride()
         p = t.data_ptr()
         if n < 2:
             s0 = heads * d
         if s2 == 1 and (s1 == d or heads == 1) and s0 >= heads * d and not (p | s0 * dtype.itemsize) & 15:
             return p, s0
-    raise _bad(name, t, f"a {dtype} [{n}, {heads}, {d}] tensor on {dev}, head rows contiguous, tokens a multiple of "
-                        "16 bytes apart, 16-byte aligned")
+    raise _bad(name, t, f"a {dtype} [{n}, {heads}, {d}] tensor on cuda:{gpu}, head rows contiguous, tokens a multiple "
+                        "of 16 bytes apart, 16-byte aligned")
+
+
+def _angles(name, t, rows, d, gpu):
+    if (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.shape == (rows, d) and rows
+            and t.get_device() == gpu and t.is_contiguous()):
+        p = t.data_ptr()
+        if not p & 15:
+            return p
+    raise _bad(name, t, f"a contiguous float32 [max_positions, {d}] tensor on cuda:{gpu}, 16-byte aligned")
 
 
 def _out(name, t, like, shape, dtype):
@@ -81,13 +97,13 @@ def _out(name, t, like, shape, dtype):
     return t
 
 
-def _enqueue(what, fn, index, *args):
-    """Calls a library entry on the current stream of device ``index``, with that device current."""
-    if torch.cuda.current_device() == index:
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+def _enqueue(what, fn, gpu, *args):
+    """Calls a library entry on the current stream of device ``gpu``, with that device current."""
+    if torch.cuda.current_device() == gpu:
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
     else:
-        with torch.cuda.device(index):
-            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        with torch.cuda.device(gpu):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
     if code:
         check(code, what)
 
@@ -154,7 +170,7 @@ class PagedKVCache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.dtype, self.device = k.dtype, k.device
-        self._index = k.device.index
+        self._gpu = k.device.index
         self._lib = lib = load_library()
         self._append, self._read, self._attend = lib.tl_paged_append, lib.tl_paged_read, lib.tl_paged_attn_decode
         ptr = [t.data_ptr() if t is not None else None for t in (k, v, k_scale, v_scale)]
@@ -166,7 +182,7 @@ class PagedKVCache:
 
     # ---------------------------------------------------------------- calls
     def _table(self, t):
-        if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 2 and t.device == self.device:
+        if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 2 and t.get_device() == self._gpu:
             n, m = t.shape
             stride, one = t.stride()
             if n < 2:
@@ -192,36 +208,32 @@ class PagedKVCache:
         """
         if not isinstance(k, torch.Tensor) or k.dim() != 3 or k.dtype not in _FLOAT_CODES:
             raise _bad("k", k, "a float32, bfloat16 or float16 [tokens, kv_heads, head_dim] tensor")
-        n, dt, dev, d = k.shape[0], k.dtype, self.device, self.head_dim
-        kp, ks = _rows("k", k, n, self.kv_heads, d, dt, dev)
-        vp, vs = _rows("v", v, n, self.kv_heads, d, dt, dev)
-        tab = self._table(block_table)
-        sp, pp = _index("seq", seq, n, dev), _index("pos", pos, n, dev)
-        if (cos is None) != (sin is None):
-            raise ValueError("cos and sin go together")
-        cosp, sinp, n_ang = None, None, 0
-        if cos is not None:
-            for name, t in (("cos", cos), ("sin", sin)):
-                if not (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.dim() == 2 and t.shape[1] == d
-                        and t.shape == cos.shape and t.shape[0] and t.device == dev and t.is_contiguous()
-                        and not t.data_ptr() & 15):
-                    raise _bad(name, t, f"a contiguous float32 [max_positions, {d}] tensor on {dev}")
-            cosp, sinp, n_ang = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-        qp, qs, heads, op = None, 0, 0, None
+        n, dt, gpu, d = k.shape[0], k.dtype, self._gpu, self.head_dim
+        kp, ks = _rows("k", k, n, self.kv_heads, d, dt, gpu)
+        vp, vs = _rows("v", v, n, self.kv_heads, d, dt, gpu)
+        tp, seqs, pages, ts = self._table(block_table)
+        sp, pp = _index("seq", seq, n, gpu), _index("pos", pos, n, gpu)
+        cp = np = angles = qp = qs = heads = op = 0
+        if cos is not None or sin is not None:
+            if cos is None or sin is None:
+                raise ValueError("cos and sin go together")
+            angles = len(cos)
+            cp, np = _angles("cos", cos, angles, d, gpu), _angles("sin", sin, angles, d, gpu)
         if q is not None:
-            if cos is None:
+            if not angles:
                 raise ValueError("q needs cos and sin")
             if not isinstance(q, torch.Tensor) or q.dim() != 3 or not q.shape[1]:
                 raise _bad("q", q, "a [tokens, heads, head_dim] tensor")
             heads = q.shape[1]
-            qp, qs = _rows("q", q, n, heads, d, dt, dev)
+            qp, qs = _rows("q", q, n, heads, d, dt, gpu)
             q_out = _out("q_out", q_out, q, (n, heads, d), dt)
             op = q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
         if n:
-            _enqueue("tl_paged_append", self._append, self._index, self._ref, qp, kp, vp, _FLOAT_CODES[dt], qs, ks, vs,
-                     sp, pp, *tab, cosp, sinp, n_ang, n, heads, op)
+            _enqueue("tl_paged_append", self._append, gpu, self._ref,
+                     _APPEND.pack(qp, kp, vp, op, sp, pp, tp, cp, np, qs, ks, vs, ts, _FLOAT_CODES[dt], seqs, pages,
+                                  angles, n, heads))
         return q_out
 
     def read(self, block_table, seq, pos, dtype=None, k_out=None, v_out=None):
@@ -233,14 +245,14 @@ class PagedKVCache:
             raise ValueError(f"dtype must be one of {[str(x) for x in _FLOAT_CODES]}, got {dtype}")
         if not isinstance(seq, torch.Tensor) or seq.dim() != 1:
             raise _bad("seq", seq, "an int32 vector")
-        n, dev = seq.shape[0], self.device
-        tab = self._table(block_table)
-        sp, pp = _index("seq", seq, n, dev), _index("pos", pos, n, dev)
+        n, gpu = seq.shape[0], self._gpu
+        tp, seqs, pages, ts = self._table(block_table)
+        sp, pp = _index("seq", seq, n, gpu), _index("pos", pos, n, gpu)
         shape = (n, self.kv_heads, self.head_dim)
         k, v = _out("k_out", k_out, self.k, shape, dtype), _out("v_out", v_out, self.k, shape, dtype)
         if n:
-            _enqueue("tl_paged_read", self._read, self._index, self._ref, sp, pp, *tab, n, k.data_ptr(), v.data_ptr(),
-                     _FLOAT_CODES[dtype])
+            _enqueue("tl_paged_read", self._read, gpu, self._ref,
+                     _READ.pack(sp, pp, tp, k.data_ptr(), v.data_ptr(), ts, seqs, pages, n, _FLOAT_CODES[dtype]))
         return k, v
 
     def attend(self, q, block_table, lengths, seq=None, sm_scale=None, out=None, return_lse=False, lse=None):
@@ -258,27 +270,27 @@ class PagedKVCache:
         if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.dtype not in _FLOAT_CODES:
             raise _bad("q", q, "a float32, bfloat16 or float16 [rows, heads, head_dim] tensor")
         n, heads, d = q.shape
-        dt, dev = q.dtype, self.device
+        dt, gpu = q.dtype, self._gpu
         if d != self.head_dim or not heads or heads % self.kv_heads:
             raise ValueError(f"q has {heads} heads of {d}: the pool has {self.kv_heads} heads of {self.head_dim}, and "
                              "q's must be a multiple")
-        qp, qs = _rows("q", q, n, heads, d, dt, dev)
-        tab = self._table(block_table)
-        lp = _index("lengths", lengths, n, dev)
+        qp, qs = _rows("q", q, n, heads, d, dt, gpu)
+        tp, seqs, pages, ts = self._table(block_table)
+        lp = _index("lengths", lengths, n, gpu)
+        sp = 0
         if seq is not None:
-            sp = _index("seq", seq, n, dev)
-        elif n > tab[1]:
-            raise ValueError(f"{n} rows but the table has {tab[1]} sequences: pass seq")
-        else:
-            sp = None
+            sp = _index("seq", seq, n, gpu)
+        elif n > seqs:
+            raise ValueError(f"{n} rows but the table has {seqs} sequences: pass seq")
         out = _out("out", out, q, (n, heads, d), dt)
         if return_lse or lse is not None:
             lse = _out("lse", lse, q, (n, heads), torch.float32)
         if n:
             work = self._workspace(heads)
-            _enqueue("tl_paged_attn_decode", self._attend, self._index, self._ref, qp, _FLOAT_CODES[dt], qs, sp, lp,
-                     *tab, n, heads, self._scale if sm_scale is None else float(sm_scale), out.data_ptr(),
-                     lse.data_ptr() if lse is not None else None, work, self._work_bytes)
+            _enqueue("tl_paged_attn_decode", self._attend, gpu, self._ref,
+                     _ATTEND.pack(qp, sp, lp, tp, out.data_ptr(), 0 if lse is None else lse.data_ptr(), work,
+                                  self._work_bytes, qs, ts, _FLOAT_CODES[dt], seqs, pages, n, heads,
+                                  self._scale if sm_scale is None else sm_scale))
         return (out, lse) if return_lse else out
 
     def _workspace(self, heads):
@@ -322,7 +334,8 @@ def token_logprobs(logits, tokens=None, top_k: int = 0) -> TokenLogprobs:
         raise _bad("logits", logits, "rows that do not overlap")
     if not 0 <= top_k <= TOP_K_MAX:
         raise ValueError(f"top_k must be in 0..{TOP_K_MAX}, got {top_k}")
-    tp = _index("tokens", tokens, n, dev) if tokens is not None else None
+    gpu = dev.index
+    tp = 0 if tokens is None else _index("tokens", tokens, n, gpu)
     f32 = torch.float32
     # the float32 results share one allocation
     if tokens is None:
@@ -333,7 +346,7 @@ def token_logprobs(logits, tokens=None, top_k: int = 0) -> TokenLogprobs:
     top = top.view(n, top_k)
     ids = logits.new_empty((n, top_k), dtype=torch.int32)
     if n:
-        _enqueue("tl_token_logprobs", load_library().tl_token_logprobs, dev.index, logits.data_ptr(),
-                 _FLOAT_CODES[logits.dtype], stride, tp, n, vocab, top_k, lp.data_ptr() if lp is not None else None,
-                 ent.data_ptr(), ids.data_ptr() if top_k else None, top.data_ptr() if top_k else None)
+        _enqueue("tl_token_logprobs", load_library().tl_token_logprobs, gpu,
+                 _LOGPROBS.pack(logits.data_ptr(), tp, 0 if lp is None else lp.data_ptr(), ent.data_ptr(),
+                                ids.data_ptr(), top.data_ptr(), stride, _FLOAT_CODES[logits.dtype], n, vocab, top_k))
     return TokenLogprobs(lp, ent, ids, top)

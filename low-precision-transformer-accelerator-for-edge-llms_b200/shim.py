@@ -152,7 +152,7 @@ def load_library(path: Path | str | None = None):
         raise ImportError(f"{p} not found: build it with build.py (nvcc, sm_100a); "
                           "there is no CPU fallback")
     lib = C.CDLL(str(p))
-    vp, i32, i64, u32, u64 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint32, C.c_uint64
+    vp, i32, u32, u64 = C.c_void_p, C.c_int32, C.c_uint32, C.c_uint64
     sig = {
         "tl_status_string": (C.c_char_p, [i32]),
         "tl_version": (i32, []),
@@ -199,13 +199,11 @@ def load_library(path: Path | str | None = None):
         "tl_contract_softmax": (i32, [vp, i32, i32, u32, vp, vp, vp]),
         "tl_contract_rope": (i32, [vp, vp, vp, i32, vp, vp]),
         "tl_residual_add_i32": (i32, [vp, vp, vp, C.c_int64, vp]),
-        "tl_paged_append": (i32, [vp, vp, vp, vp, i32, i64, i64, i64, vp, vp, vp, i32, i32, i64, vp, vp, i32, i32, i32,
-                                  vp, vp]),
-        "tl_paged_read": (i32, [vp, vp, vp, vp, i32, i32, i64, i32, vp, vp, i32, vp]),
+        "tl_paged_append": (i32, [vp, vp, vp]),
+        "tl_paged_read": (i32, [vp, vp, vp]),
         "tl_paged_attn_workspace_bytes": (C.c_size_t, [i32, i32, i32]),
-        "tl_paged_attn_decode": (i32, [vp, vp, i32, i64, vp, vp, vp, i32, i32, i64, i32, i32, C.c_float, vp, vp, vp,
-                                       C.c_size_t, vp]),
-        "tl_token_logprobs": (i32, [vp, i32, i64, vp, i32, i32, i32, vp, vp, vp, vp, vp]),
+        "tl_paged_attn_decode": (i32, [vp, vp, vp]),
+        "tl_token_logprobs": (i32, [vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

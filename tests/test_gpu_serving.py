@@ -591,21 +591,23 @@ def test_c_entry_refuses_bad_arguments(pkg):
     one = i32([1])
     need = lib.tl_paged_attn_workspace_bytes(4, 2, 64)
     work = torch.zeros(need, dtype=torch.uint8, device="cuda")
-    good = dict(cache=c._ref, q=q.data_ptr(), dt=0, qs=256, seq=one.data_ptr(), le=one.data_ptr(),
-                tab=table.data_ptr(), n=1, mp=2, ts=2, rows=1, heads=4, sc=0.125, out=q.data_ptr(), lse=None,
-                w=work.data_ptr(), wb=need, st=None)
     out = torch.empty_like(q)
-    good["out"] = out.data_ptr()
+    good = dict(q=q.data_ptr(), seq=one.data_ptr(), le=one.data_ptr(), tab=table.data_ptr(), out=out.data_ptr(), lse=0,
+                w=work.data_ptr(), wb=need, qs=256, ts=2, dt=0, n=1, mp=2, rows=1, heads=4, sc=0.125)
 
-    def call(**kw):
-        return lib.tl_paged_attn_decode(*{**good, **kw}.values())
+    def call(cache=c._ref, **kw):
+        return lib.tl_paged_attn_decode(cache, pkg.serving._ATTEND.pack(*{**good, **kw}.values()), None)
 
     assert call() == 0
-    for kw in (dict(cache=None), dict(q=None), dict(dt=3), dict(dt=9), dict(qs=255), dict(qs=128), dict(le=None),
-               dict(tab=None), dict(n=0), dict(mp=0), dict(ts=1), dict(rows=0), dict(heads=3), dict(heads=0),
-               dict(out=None), dict(w=None), dict(q=q.data_ptr() + 4)):
+    assert call(cache=None) == 16 and lib.tl_paged_attn_decode(c._ref, None, None) == 16
+    for kw in (dict(q=0), dict(dt=3), dict(dt=9), dict(qs=255), dict(qs=128), dict(le=0), dict(tab=0), dict(n=0),
+               dict(mp=0), dict(ts=1), dict(rows=0), dict(heads=3), dict(heads=0), dict(out=0), dict(w=0),
+               dict(q=q.data_ptr() + 4)):
         assert call(**kw) == 16, kw
-    assert call(wb=need - 1) == 17 and call(seq=None, rows=2) == 17 and call(mp=2**30, ts=2**30) == 17
+    assert call(wb=need - 1) == 17 and call(seq=0, rows=2) == 17 and call(mp=2**30, ts=2**30) == 17
+    for fn in (lib.tl_paged_append, lib.tl_paged_read):
+        assert fn(c._ref, None, None) == 16 and fn(None, b"\0" * 256, None) == 16 and fn(c._ref, b"\0" * 256, None) == 16
+    assert lib.tl_token_logprobs(None, None) == 16 and lib.tl_token_logprobs(b"\0" * 256, None) == 16
     for h, kv, d in ((0, 1, 64), (4, 0, 64), (5, 2, 64), (4, 2, 80)):
         assert lib.tl_paged_attn_workspace_bytes(h, kv, d) == 0
     torch.cuda.synchronize()
