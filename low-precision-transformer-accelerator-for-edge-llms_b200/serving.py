@@ -90,6 +90,8 @@ def _angles(name, t, rows, d, gpu):
 def _out(name, t, like, shape, dtype):
     """``t`` checked as a contiguous output on ``like``'s device, or a new tensor."""
     if t is None:
+        if like.dtype is dtype and like.shape == shape:
+            return torch.empty_like(like, memory_format=torch.contiguous_format)
         return like.new_empty(shape, dtype=dtype)
     if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == like.device
             and t.is_contiguous() and not t.data_ptr() & 15):
@@ -217,7 +219,7 @@ class PagedKVCache:
         if cos is not None or sin is not None:
             if cos is None or sin is None:
                 raise ValueError("cos and sin go together")
-            angles = len(cos)
+            angles = cos.shape[0]
             cp, np = _angles("cos", cos, angles, d, gpu), _angles("sin", sin, angles, d, gpu)
         if q is not None:
             if not angles:
