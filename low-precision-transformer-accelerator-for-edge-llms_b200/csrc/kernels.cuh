@@ -187,8 +187,9 @@ int attn_splits(int M, int Hkv, int P);
 size_t attn_part_floats(int M, int Hkv, int P);
 cudaError_t attn_prepare();
 cudaError_t attn_read_error(unsigned int* code);
-// The same for the paged attention kernel (paged_attn.cu).
+// The same for the paged attention (paged_attn.cu) and log-probability (logprobs.cu) kernels.
 cudaError_t paged_attn_read_error(unsigned int* code);
+cudaError_t logprob_read_error(unsigned int* code);
 
 // ---- prefill helpers (rows of n_seq sequences of seq_len tokens each)
 cudaError_t launch_embed(const float* table, const int* ids, float* x, int rows, int D,

@@ -17,10 +17,11 @@
 // values: the lower index is the larger key), which makes every choice below
 // unique: the list does not depend on the order in which threads find it.
 //
-// What bounds it: reading the logits. Each thread has several 16-byte loads
-// in flight, and a row is split over the CTAs of a cluster, which join their
-// sums and lists through distributed shared memory, while rows are too few
-// for the SMs.
+// What bounds it: reading the logits. A warp's tiles arrive by bulk copies a
+// few tiles ahead. Few rows are split over the CTAs of a cluster, which join
+// their sums and lists through distributed shared memory. Many rows go to
+// persistent CTAs in which two warps put a row's results together (a chain of
+// short steps that reads little) while the others sum the next row.
 #include <algorithm>
 #include <cfloat>
 #include <type_traits>
@@ -32,14 +33,28 @@
 namespace tl {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kUnroll = 4;      // 16-byte loads of a thread in flight
+constexpr int kUnroll = 4;        // 16-byte pieces of a thread in a tile
+constexpr int kTile = kUnroll * 32, kTileBytes = kTile * 16;  // pieces and bytes of a warp's tile
+// Tiles of a warp under way, warps of a CTA that sum rows, that put results
+// together, and such CTAs an SM holds. 2048 rows of 32000 float32 take 47.8 us
+// (5.5 TB/s) with 2, 8, 2, 3; with four tiles under way 54.9 (SMs drift apart:
+// the rows are handed out beforehand), with one result warp 65.5, with two
+// CTAs of 8 + 2 or 8 + 4 warps 50.9 and 51.2, and 52 to 57 where all warps of
+// a CTA work on the results between rows.
+constexpr int kStages = 2;
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kPostWarps = 2;
+constexpr int kRowCtas = 3;
 constexpr int kCandidates = 512;
 constexpr int kMaxCluster = 8;
 constexpr int kPicks = TL_TOP_K_MAX / kWarps + 1;  // largest maxima taken of a warp
+constexpr int kRing = kWarps * kStages * kTileBytes;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 using Key = unsigned long long;
+
+// Set when a wait on a tile ran out (tl_device_error reads and clears it).
+__device__ unsigned int g_logprob_error = 0;
 
 struct LogprobArgs {
   const void* x;
@@ -61,6 +76,38 @@ TL_DEV float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+TL_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two float32 operations in one instruction; a pair is 64 bits.
+using Pair = unsigned long long;
+TL_DEV Pair pair(float x, float y) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+  return p;
+}
+TL_DEV float2 halves(Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+TL_DEV Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+TL_DEV Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+TL_DEV Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 TL_DEV unsigned redux_max(unsigned v) { return __reduce_max_sync(0xffffffffu, v); }
 TL_DEV Key warp_max_key(Key k) {
   const unsigned hi = redux_max(static_cast<unsigned>(k >> 32));
@@ -72,17 +119,15 @@ TL_DEV Key warp_max_key(Key k) {
 struct Sums {
   float m, s, t;
 };
-TL_DEV Sums join(const Sums& a, const Sums& b) {
-  Sums r;
-  r.m = fmaxf(a.m, b.m);
-  const float ea = (a.m - r.m) * kLog2e, eb = (b.m - r.m) * kLog2e;
-  const float fa = ex2(ea), fb = ex2(eb);
+// Joins the sums of the lanes of a warp.
+TL_DEV Sums warp_join(Sums a) {
+  const float m = warp_max(a.m);
+  const float e = (a.m - m) * kLog2e, f = ex2(e);
   // a factor that underflows takes its (possibly infinite) exponent with it
-  r.s = fa * a.s + fb * b.s;
-  r.t = (fa > 0.0f ? fa * (a.t + ea * a.s) : 0.0f * a.s) + (fb > 0.0f ? fb * (b.t + eb * b.s) : 0.0f * b.s);
-  return r;
+  a.t = f > 0.0f ? f * (a.t + e * a.s) : 0.0f * a.s;
+  a.s = f * a.s;
+  return {m, warp_sum(a.s), warp_sum(a.t)};
 }
-
 template <typename T>
 struct Chunk {
   static constexpr int N = 16 / sizeof(T);
@@ -92,6 +137,7 @@ struct Chunk {
                  : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                  : "l"(p));
   }
+  TL_DEV void load_shared(const unsigned char* p) { w = *reinterpret_cast<const uint4*>(p); }
   TL_DEV void get(float* x) const {
     const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -112,132 +158,219 @@ struct Chunk {
 
 // A thread's running sums and its largest element.
 struct Running {
-  Sums a{-FLT_MAX, 0.0f, 0.0f};
+  float m = -FLT_MAX;              // the sums' reference
+  Pair s = 0, t = 0;               // even and odd elements
   float best = -INFINITY;
   int at = 0;  // an index not below the largest element's
 
-  template <int N>
-  TL_DEV void add(const float* x, int last) {
-    float top = x[0];
+  // The reference follows only when sums would grow past 2^29 of it.
+  TL_DEV void follow(float top) {
+    if (top > m + 20.0f) {
+      const float e = (m - top) * kLog2e, f = ex2(e);
+      const Pair f2 = pair(f, f);
+      t = f > 0.0f ? mul2(f2, fma2(pair(e, e), s, t)) : 0;
+      s = mul2(f2, s);
+      m = top;
+    }
+  }
+  // B batches of N elements, the last of batch b at index last + b * step.
+  template <int B, int N>
+  TL_DEV void add(const float (&x)[B][N], int last, int step) {
+    float top[B];
 #pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
-    if (top > best) {
-      best = top;
-      at = last;
-      // the reference follows only when sums would grow past 2^30 of it
-      if (top > a.m + 20.0f) {
-        const float e = (a.m - top) * kLog2e, f = ex2(e);
-        a.t = f > 0.0f ? f * (a.t + e * a.s) : 0.0f;
-        a.s *= f;
-        a.m = top;
+    for (int b = 0; b < B; ++b) {
+      top[b] = N == 1 ? x[b][0] : fmaxf(x[b][0], x[b][N - 1]);
+#pragma unroll
+      for (int i = 1; i + 1 < N; i += 2) top[b] = max3(top[b], x[b][i], x[b][i + 1]);
+    }
+    float most = top[0];
+#pragma unroll
+    for (int b = 1; b < B; ++b) most = fmaxf(most, top[b]);
+    if (most > best) {
+      best = most;
+      int first = B - 1;
+#pragma unroll
+      for (int b = B - 2; b >= 0; --b) first = top[b] == most ? b : first;
+      at = last + first * step;
+      follow(most);
+    }
+    const Pair mm = pair(-m, -m), log2e = pair(kLog2e, kLog2e);
+    Pair s1 = 0, t1 = 0;
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int i = 0; i < N; i += 2) {
+        // (a single element pairs with -infinity)
+        const Pair y = mul2(add2(pair(x[b][i], i + 1 < N ? x[b][i + 1 < N ? i + 1 : 0] : -INFINITY), mm), log2e);
+        const float2 v = halves(y);
+        const Pair e = pair(ex2(v.x), ex2(v.y));  // NaN and infinity stay in the sums and mark the row
+        s1 = add2(s1, e);
+        t1 = fma2(e, y, t1);
       }
-    }
+    const float2 tt = halves(t1);
+    if (!(tt.x + tt.y > -INFINITY)) {
+      // 0 times -infinity among the terms (or a NaN that stays one): again, with y bounded
+      t1 = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float y = (x[i] - a.m) * kLog2e;
-      const float e = ex2(y);  // NaN and infinity stay in the sums and mark the row
-      a.s += e;
-      a.t = fmaf(e, fmaxf(y, -200.0f), a.t);  // 0 times a finite number for -infinity
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float y = (x[b][i] - m) * kLog2e;
+          t1 = add2(t1, pair(ex2(y) * fmaxf(y, -200.0f), 0.0f));
+        }
     }
+    s = add2(s, s1);
+    t = add2(t, t1);
+  }
+  TL_DEV Sums sums() const {
+    const float2 a = halves(s), b = halves(t);
+    return {m, a.x + a.y, b.x + b.y};
   }
 };
 
-struct Shared {
+// What the summing warps leave of a row.
+struct RowSums {
   Sums sums[kWarps];
-  Key picks[kWarps * kPicks];
+  Key picks[kWarps * kPicks];  // of each warp, its largest groups' maxima
+  Key best[kThreads];          // every group's maximum
+};
+struct Shared {
+  RowSums row[2];
   Key cand[kCandidates];
   Key list[TL_TOP_K_MAX];  // this CTA's largest, in order, then zeros
-  Sums row;                // this CTA's sums
+  Sums total;              // this CTA's sums
   int groups[kThreads];
   int n_groups, n_cand;
   Key reduce[kWarps];
+  uint64_t tiles[kWarps * kStages], full[2], empty[2];  // barriers
 };
 
-// The CTA's share of a row: elements before the first 16-byte boundary and
-// after the last whole chunk belong to the threads of CTA 0, chunks to CTA
-// (i / kThreads) % ctas.
+// The CTA's share of a row. Whole 16-byte pieces are cut into tiles of kTile,
+// which go to the warps of all CTAs in turn; lane l has pieces l, l + 32, ...
+// of a tile. Elements before the first 16-byte boundary and after the last
+// whole piece belong to the first threads of CTA 0.
 template <typename T>
 struct Share {
+  static constexpr int N = Chunk<T>::N;
   const T* x;
   int vocab, head, chunks, ctas, rank;
-  TL_DEV int chunk_first(int i) const { return head + i * Chunk<T>::N; }
-  TL_DEV int first_of(int thread) const { return rank * kThreads + thread; }
-  TL_DEV int stride() const { return ctas * kThreads; }
+  TL_DEV int chunk_first(int i) const { return head + i * N; }
+  TL_DEV int tiles() const { return (chunks + kTile - 1) / kTile; }
+  TL_DEV int tile(int warp, int i) const { return rank * kWarps + warp + i * step(); }  // warp's i-th tile
+  TL_DEV int step() const { return ctas * kWarps; }
   // the loose element of a thread, -1: none
   TL_DEV int loose(int thread) const {
     if (rank) return -1;
-    const int i = thread < Chunk<T>::N ? thread : chunk_first(chunks) + thread - Chunk<T>::N;
-    return thread < Chunk<T>::N ? (i < head ? i : -1) : i < vocab ? i : -1;
+    const int i = thread < N ? thread : chunk_first(chunks) + thread - N;
+    return thread < N ? (i < head ? i : -1) : i < vocab ? i : -1;
   }
 };
 
+// The threads that put results together: all of the CTA, or the last PT.
+template <int PT>
+struct Post {
+  TL_DEV static int tid() { return PT == kThreads ? threadIdx.x : threadIdx.x - kThreads; }
+  TL_DEV static void sync() {
+    if constexpr (PT == kThreads)
+      __syncthreads();
+    else
+      asm volatile("bar.sync 1, %0;" ::"n"(PT) : "memory");
+  }
+};
+
+// A warp's part of what is left of a row.
+TL_DEV void leave(const Running& run, int top_k, RowSums& row) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Sums sum = warp_join(run.sums());
+  if (lane == 0) row.sums[warp] = sum;
+  if (!top_k) return;
+  const Key mine = run.best > -INFINITY ? argmax_key(run.best + 0.0f, run.at) : 0;
+  row.best[threadIdx.x] = mine;
+  const int picks = (top_k + kWarps - 1) / kWarps + 1;
+  Key left = mine;
+  for (int i = 0; i < picks; ++i) {
+    const Key top = warp_max_key(left);
+    if (left == top) left = 0;  // keys of two lanes differ unless both are empty
+    if (lane == 0) row.picks[warp * picks + i] = top;
+  }
+}
+
 // Writes the `k` largest keys of sh.cand[0..n) to sh.list in order (zeros
 // behind): an element's place is the number of larger ones.
+template <int PT>
 TL_DEV void order_candidates(Shared& sh, int n, int k) {
-  if (threadIdx.x < TL_TOP_K_MAX) sh.list[threadIdx.x] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
+  const int tid = Post<PT>::tid();
+  if (tid < TL_TOP_K_MAX) sh.list[tid] = 0;
+  Post<PT>::sync();
+  for (int i = tid; i < n; i += PT) {
     const Key mine = sh.cand[i];
     int place = 0;
     for (int j = 0; j < n; ++j) place += sh.cand[j] > mine;
     if (place < k) sh.list[place] = mine;
   }
-  __syncthreads();
+  Post<PT>::sync();
 }
 
 // The k largest keys of the CTA's share -> sh.list.
-template <typename T>
-__device__ void top_of_share(const Share<T>& w, const Running& run, int k, Shared& sh) {
-  constexpr int N = Chunk<T>::N;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int picks = (k + kWarps - 1) / kWarps + 1;
-  const Key mine = run.best > -INFINITY ? argmax_key(run.best + 0.0f, run.at) : 0;
+template <typename T, int PT>
+__device__ void top_of_share(const Share<T>& w, const RowSums& row, int k, Shared& sh) {
+  constexpr int N = Chunk<T>::N, PW = PT / 32;
+  const int tid = Post<PT>::tid(), lane = tid & 31, warp = tid >> 5;
+  const int n_picks = kWarps * ((k + kWarps - 1) / kWarps + 1);
   if (tid == 0) sh.n_groups = sh.n_cand = 0;
-  {
-    Key left = mine;
-    for (int i = 0; i < picks; ++i) {
-      const Key top = warp_max_key(left);
-      if (left == top) left = 0;  // keys of two lanes differ unless both are empty
-      if (lane == 0) sh.picks[warp * picks + i] = top;
-    }
-  }
-  __syncthreads();
   // the k-th largest of the picks (0 if there are fewer)
   Key bar = ~0ull;
-  for (int i = lane; i < kWarps * picks; i += 32) {
-    const Key p = sh.picks[i];
+  for (int i = lane; i < n_picks; i += 32) {
+    const Key p = row.picks[i];
     int above = 0;
-    for (int j = 0; j < kWarps * picks; ++j) above += sh.picks[j] > p;
+    for (int j = 0; j < n_picks; ++j) above += row.picks[j] > p;
     if (above < k && p < bar) bar = p;
   }
   bar = ~warp_max_key(~bar);
-  if (mine && mine >= bar) sh.groups[atomicAdd(&sh.n_groups, 1)] = tid;
-  __syncthreads();
+  Post<PT>::sync();
+  for (int g = tid; g < kThreads; g += PT)
+    if (row.best[g] && row.best[g] >= bar) sh.groups[atomicAdd(&sh.n_groups, 1)] = g;
+  Post<PT>::sync();
   const int n_groups = sh.n_groups;
+  const float bar_value = bar ? key_value(bar) : -INFINITY;
   auto offer = [&](float v, int i) {
-    if (!(v > -INFINITY)) return;
+    if (!(v >= bar_value && v > -INFINITY)) return;
     const Key key = argmax_key(v + 0.0f, i);
     if (key < bar) return;
     const int at = atomicAdd(&sh.n_cand, 1);
     if (at < kCandidates) sh.cand[at] = key;
   };
-  for (int gi = warp; gi < n_groups; gi += kWarps) {
-    const int g = sh.groups[gi];
-    for (int c = w.first_of(g) + lane * w.stride(); c < w.chunks; c += 32 * w.stride()) {
-      Chunk<T> y;
-      float v[N];
-      y.load(w.x + w.chunk_first(c));
-      y.get(v);
+  // the groups' pieces, spread over the threads, a few loads in flight
+  const int per = (w.tiles() + w.step() - 1) / w.step() * kUnroll, pieces = n_groups * per;
+  constexpr int F = PT == kThreads ? 1 : 4;
+  for (int i0 = tid; i0 < pieces; i0 += PT * F) {
+    Chunk<T> y[F];
+    int c[F];
 #pragma unroll
-      for (int i = 0; i < N; ++i) offer(v[i], w.chunk_first(c) + i);
+    for (int f = 0; f < F; ++f) {
+      const int i = i0 + f * PT;
+      c[f] = w.chunks;
+      if (i < pieces) {
+        const int g = sh.groups[i / per], place = i % per;
+        c[f] = w.tile(g >> 5, place / kUnroll) * kTile + place % kUnroll * 32 + (g & 31);
+      }
+      if (c[f] < w.chunks) y[f].load(w.x + w.chunk_first(c[f]));
     }
-    const int loose = w.loose(g);
-    if (lane == 0 && loose >= 0) offer(to_f32(w.x[loose]), loose);
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+      if (c[f] < w.chunks) {
+        float v[N];
+        y[f].get(v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) offer(v[e], w.chunk_first(c[f]) + e);
+      }
   }
-  __syncthreads();
+  for (int i = tid; i < n_groups; i += PT)
+    if (const int loose = w.loose(sh.groups[i]); loose >= 0) offer(to_f32(w.x[loose]), loose);
+  Post<PT>::sync();
   const int n = sh.n_cand;
   if (n <= kCandidates) {
-    order_candidates(sh, n, k);
+    order_candidates<PT>(sh, n, k);
     return;
   }
   // A few groups hold more large elements than there is room for: take the
@@ -250,26 +383,31 @@ __device__ void top_of_share(const Share<T>& w, const Running& run, int k, Share
       const Key key = v > -INFINITY ? argmax_key(v + 0.0f, i) : 0;
       if (key < last && key > top) top = key;
     };
-    for (int c = w.first_of(tid); c < w.chunks; c += w.stride()) {
-      Chunk<T> y;
-      float v[N];
-      y.load(w.x + w.chunk_first(c));
-      y.get(v);
+    for (int g = tid; g < kThreads; g += PT) {
+      for (int i = 0; w.tile(g >> 5, i) < w.tiles(); ++i)
+        for (int u = 0; u < kUnroll; ++u) {
+          const int c = w.tile(g >> 5, i) * kTile + u * 32 + (g & 31);
+          if (c >= w.chunks) break;
+          Chunk<T> y;
+          float v[N];
+          y.load(w.x + w.chunk_first(c));
+          y.get(v);
 #pragma unroll
-      for (int i = 0; i < N; ++i) see(v[i], w.chunk_first(c) + i);
+          for (int e = 0; e < N; ++e) see(v[e], w.chunk_first(c) + e);
+        }
+      const int loose = w.loose(g);
+      if (loose >= 0) see(to_f32(w.x[loose]), loose);
     }
-    const int loose = w.loose(tid);
-    if (loose >= 0) see(to_f32(w.x[loose]), loose);
     top = warp_max_key(top);
-    __syncthreads();
+    Post<PT>::sync();
     if (lane == 0) sh.reduce[warp] = top;
-    __syncthreads();
-    for (int i = 0; i < kWarps; ++i) top = sh.reduce[i] > top ? sh.reduce[i] : top;
+    Post<PT>::sync();
+    for (int i = 0; i < PW; ++i) top = sh.reduce[i] > top ? sh.reduce[i] : top;
     if (top == 0) break;
     if (tid == 0) sh.list[r] = top;
     last = top;
   }
-  __syncthreads();
+  Post<PT>::sync();
 }
 
 TL_DEV uint32_t peer_address(const void* p, unsigned rank) {
@@ -288,128 +426,223 @@ TL_DEV Key peer_key(const Key* p, unsigned rank) {
   return v;
 }
 
-template <typename T, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads) logprob_kernel(const __grid_constant__ LogprobArgs a, int ctas) {
-  constexpr int N = Chunk<T>::N;
-  __shared__ Shared sh;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r = CLUSTER ? blockIdx.x / ctas : blockIdx.x;
-  Share<T> w;
-  w.x = static_cast<const T*>(a.x) + r * a.ld;
-  w.vocab = a.vocab;
-  w.head = min(a.vocab, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(w.x) & 15)) % 16 / sizeof(T)));
-  w.chunks = (a.vocab - w.head) / N;
-  w.ctas = CLUSTER ? ctas : 1;
-  w.rank = CLUSTER ? blockIdx.x % ctas : 0;
-
-  // the given token's logit, long before it is needed
-  int token = -1;
-  float given = 0.0f;
-  if (tid == 0 && w.rank == 0 && a.tokens) {
-    token = a.tokens[r];
-    if (token >= 0 && token < a.vocab) given = to_f32(w.x[token]);
-  }
-
-  // ---- one pass
-  // In ascending order, so that a thread's `at` belongs to the first of equal
-  // elements: then an element that beats the bar is in a group that does.
-  Running run;
-  const int loose = w.loose(tid);
-  if (loose >= 0 && loose < w.head) {
-    const float v = to_f32(w.x[loose]);
-    run.add<1>(&v, loose);
-  }
-  int c = w.first_of(tid);
-  const int stride = w.stride();
-  for (; c + (kUnroll - 1) * stride < w.chunks; c += kUnroll * stride) {
-    Chunk<T> y[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) y[u].load(w.x + w.chunk_first(c + u * stride));
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      float v[N];
-      y[u].get(v);
-      run.add<N>(v, w.chunk_first(c + u * stride) + N - 1);
-    }
-  }
-  for (; c < w.chunks; c += stride) {
-    Chunk<T> y;
-    float v[N];
-    y.load(w.x + w.chunk_first(c));
-    y.get(v);
-    run.add<N>(v, w.chunk_first(c) + N - 1);
-  }
-  if (loose >= w.head) {
-    const float v = to_f32(w.x[loose]);
-    run.add<1>(&v, loose);
-  }
-
-  // ---- the CTA's sums
-  Sums sum = run.a;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums other{__shfl_xor_sync(0xffffffffu, sum.m, o), __shfl_xor_sync(0xffffffffu, sum.s, o),
-                     __shfl_xor_sync(0xffffffffu, sum.t, o)};
-    sum = join(sum, other);
-  }
-  if (lane == 0) sh.sums[warp] = sum;
-  __syncthreads();
-  sum = sh.sums[0];
-  for (int i = 1; i < kWarps; ++i) sum = join(sum, sh.sums[i]);
-  if (a.top_k) top_of_share(w, run, a.top_k, sh);
-
-  if constexpr (CLUSTER) {
-    if (tid == 0) sh.row = sum;
-    cluster_sync();
-    if (w.rank == 0) {
-      for (int p = 1; p < ctas; ++p)
-        sum = join(sum, Sums{peer_float(&sh.row.m, p), peer_float(&sh.row.s, p), peer_float(&sh.row.t, p)});
-      if (a.top_k) {
-        const int n = ctas * a.top_k;  // at most 8 * 32
-        for (int i = tid; i < n; i += kThreads) sh.cand[i] = peer_key(sh.list + i % a.top_k, i / a.top_k);
-        __syncthreads();
-        order_candidates(sh, n, a.top_k);
-      }
-    }
-    cluster_sync();  // no CTA leaves while its shared memory may be read
-    if (w.rank) return;
-  }
-
-  // ---- the row's results
+// One row's results from its sums and list.
+TL_DEV void write_row(const LogprobArgs& a, int r, int tid, const Sums& sum, const Key* list, int token, float given) {
   const float nan = __int_as_float(0x7fc00000);
   const bool bad = !(sum.s < INFINITY), none = sum.s == 0.0f;
   const float ln_s = logf(sum.s);
   if (tid == 0) {
     if (a.tokens)
-      a.logprob[r] = token < 0                        ? 0.0f
-                     : bad || token >= a.vocab        ? nan
-                     : none || given == -INFINITY     ? -INFINITY
-                                                      : (given - sum.m) - ln_s;
+      a.logprob[r] = token < 0                    ? 0.0f
+                     : bad || token >= a.vocab    ? nan
+                     : none || given == -INFINITY ? -INFINITY
+                                                  : (given - sum.m) - ln_s;
     if (a.entropy) a.entropy[r] = bad ? nan : none ? 0.0f : ln_s - kLn2 * (sum.t / sum.s);
   }
   if (tid < a.top_k) {
-    const Key key = bad ? 0 : sh.list[tid];
+    const Key key = bad ? 0 : list[tid];
     const int64_t o = static_cast<int64_t>(r) * a.top_k + tid;
     a.top_ids[o] = key ? argmax_key_index(key) : -1;
     a.top_lp[o] = bad ? nan : key ? (key_value(key) - sum.m) - ln_s : -INFINITY;
   }
 }
 
+// CLUSTER: a row a cluster of `ctas` CTAs. Otherwise row blockIdx.x,
+// + gridDim.x, ... a CTA.
+template <typename T, bool CLUSTER>
+__global__ void __launch_bounds__(CLUSTER ? kThreads : kThreads + kPostWarps * 32, CLUSTER ? 2 : kRowCtas)
+    logprob_kernel(const __grid_constant__ LogprobArgs a, int ctas) {
+  constexpr int N = Chunk<T>::N;
+  extern __shared__ __align__(128) unsigned char rings[];
+  __shared__ Shared sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int first_row = CLUSTER ? blockIdx.x / ctas : blockIdx.x;
+  const int row_step = CLUSTER ? gridDim.x / ctas : gridDim.x;
+  auto share = [&](int r) {
+    Share<T> w;
+    w.x = static_cast<const T*>(a.x) + r * a.ld;
+    w.vocab = a.vocab;
+    w.head = min(a.vocab, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(w.x) & 15)) % 16 / sizeof(T)));
+    w.chunks = (a.vocab - w.head) / N;
+    w.ctas = CLUSTER ? ctas : 1;
+    w.rank = CLUSTER ? blockIdx.x % ctas : 0;
+    return w;
+  };
+  auto tiles_of = [&](const Share<T>& w) {
+    return w.tile(warp, 0) < w.tiles() ? (w.tiles() - 1 - w.tile(warp, 0)) / w.step() + 1 : 0;
+  };
+  bool late = false;  // a wait has run out: the results are void, the host learns of it
+  auto wait = [&](uint64_t* bar, int parity, unsigned code) {
+    if (late ? !mbar_try_wait(bar, parity) : !mbar_wait_err(bar, parity, code, &g_logprob_error)) late = true;
+  };
+  if (!CLUSTER && tid == 0)
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(sh.full + i, kWarps);
+      mbar_init(sh.empty + i, 1);
+    }
+  uint64_t* bars = sh.tiles + warp * kStages;
+  if (warp < kWarps && lane == 0)
+    for (int i = 0; i < kStages; ++i) mbar_init(bars + i, 1);
+  if (lane == 0) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  if constexpr (CLUSTER)
+    __syncwarp();
+  else
+    __syncthreads();
+
+  if (!CLUSTER && warp >= kWarps) {
+    // ---- results, a row behind
+    constexpr int PT = kPostWarps * 32;
+    for (int r = first_row, n = 0; r < a.rows; r += row_step, ++n) {
+      const Share<T> w = share(r);
+      const int token = a.tokens ? a.tokens[r] : -1;
+      const float given = token >= 0 && token < a.vocab ? to_f32(w.x[token]) : 0.0f;
+      const RowSums& row = sh.row[n & 1];
+      wait(sh.full + (n & 1), n >> 1 & 1, 3u);
+      const Sums sum = warp_join(lane < kWarps ? row.sums[lane] : Sums{-FLT_MAX, 0.0f, 0.0f});
+      if (a.top_k) top_of_share<T, PT>(w, row, a.top_k, sh);
+      write_row(a, r, Post<PT>::tid(), sum, sh.list, token, given);
+      Post<PT>::sync();  // the list and the row's sums have been read
+      if (Post<PT>::tid() == 0) mbar_arrive(sh.empty + (n & 1));
+    }
+    return;
+  }
+
+  // ---- the warp's ring, filled kStages tiles ahead, also across rows
+  unsigned char* ring = rings + warp * kStages * kTileBytes;
+  int fill_row = first_row, fill_i = 0, filled = 0;
+  Share<T> fill_w = share(fill_row);
+  int fill_n = tiles_of(fill_w);
+  auto fill = [&](int stage) {
+    while (fill_i >= fill_n) {
+      fill_row += row_step;
+      if (fill_row >= a.rows) return;
+      fill_w = share(fill_row);
+      fill_n = tiles_of(fill_w);
+      fill_i = 0;
+    }
+    if (lane == 0) {
+      const int first = fill_w.tile(warp, fill_i) * kTile;
+      const uint32_t bytes = min(kTile, fill_w.chunks - first) * 16;
+      mbar_arrive_expect_tx(bars + stage, bytes);
+      bulk_load(ring + stage * kTileBytes, fill_w.x + fill_w.chunk_first(first), bytes, bars + stage);
+    }
+    ++fill_i;
+    ++filled;
+  };
+  for (int i = 0; i < kStages; ++i)
+    if (fill_row < a.rows) fill(i);
+
+  int stage = 0, phase = 0;
+  for (int r = first_row, n = 0; r < a.rows; r += row_step, ++n) {
+    const Share<T> w = share(r);
+    const int n_tiles = tiles_of(w);
+    int token = -1;
+    float given = 0.0f;
+    if (CLUSTER && tid == 0 && w.rank == 0 && a.tokens) {
+      token = a.tokens[r];
+      if (token >= 0 && token < a.vocab) given = to_f32(w.x[token]);
+    }
+    // In ascending order, so that a thread's `at` belongs to the first of equal
+    // elements: then an element that beats the bar is in a group that does.
+    Running run;
+    const int loose = w.loose(tid);
+    if (loose >= 0 && loose < w.head) {
+      const float v[1][1] = {{to_f32(w.x[loose])}};
+      run.add(v, loose, 0);
+    }
+    for (int i = 0; i < n_tiles; ++i) {
+      const int first = w.tile(warp, i) * kTile;
+      const int pieces = min(kTile, w.chunks - first);
+      wait(bars + stage, phase, 1u);
+      Chunk<T> y[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) y[u].load_shared(ring + stage * kTileBytes + (u * 32 + lane) * 16);
+      __syncwarp();
+      if (fill_row < a.rows) fill(stage);
+      if (pieces == kTile) {
+        float v[kUnroll][N];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) y[u].get(v[u]);
+        run.add(v, w.chunk_first(first + lane) + N - 1, 32 * N);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (u * 32 + lane < pieces) {
+            float v[1][N];
+            y[u].get(v[0]);
+            run.add(v, w.chunk_first(first + u * 32 + lane) + N - 1, 0);
+          }
+      }
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    if (loose >= w.head) {
+      const float v[1][1] = {{to_f32(w.x[loose])}};
+      run.add(v, loose, 0);
+    }
+
+    if constexpr (!CLUSTER) {
+      wait(sh.empty + (n & 1), (n >> 1 & 1) ^ 1, 4u);
+      leave(run, a.top_k, sh.row[n & 1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sh.full + (n & 1));
+    } else {
+      leave(run, a.top_k, sh.row[0]);
+      __syncthreads();
+      // (every warp joins the warps' sums; lanes beyond them bring nothing)
+      Sums sum = warp_join(lane < kWarps ? sh.row[0].sums[lane] : Sums{-FLT_MAX, 0.0f, 0.0f});
+      if (a.top_k) top_of_share<T, kThreads>(w, sh.row[0], a.top_k, sh);
+      if (tid == 0) sh.total = sum;
+      cluster_sync();
+      if (w.rank == 0) {
+        // peers' lists and sums in one round of remote loads
+        const int m = ctas * a.top_k;  // at most 8 * 32
+        if (tid < m) sh.cand[tid] = peer_key(sh.list + tid % a.top_k, tid / a.top_k);
+        Sums part{-FLT_MAX, 0.0f, 0.0f};
+        if (lane < ctas)
+          part = {peer_float(&sh.total.m, lane), peer_float(&sh.total.s, lane), peer_float(&sh.total.t, lane)};
+        sum = warp_join(part);
+        __syncthreads();
+        if (a.top_k) order_candidates<kThreads>(sh, m, a.top_k);
+        write_row(a, r, tid, sum, sh.list, token, given);
+      }
+      cluster_sync();  // no CTA goes on while its shared memory may be read
+    }
+  }
+  if (late)  // copies still under way must not land after the CTA has gone
+    for (int i = max(0, filled - kStages); i < filled; ++i)
+      mbar_wait_err(bars + i % kStages, i / kStages & 1, 2u, &g_logprob_error);
+}
+
 template <typename T>
 tl_status logprob_launch(const LogprobArgs& a, cudaStream_t s) {
-  // A row is split over a cluster while CTAs of whole rows would leave SMs
-  // without work, down to one round of loads a thread.
+  static bool ready[64];  // once a device: the rings need more shared memory than the default limit
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TL_ERR_CUDA;
+  if (!ready[dev]) {
+    if (cudaFuncSetAttribute(logprob_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing) !=
+            cudaSuccess ||
+        cudaFuncSetAttribute(logprob_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing) != cudaSuccess)
+      return TL_ERR_CUDA;
+    ready[dev] = true;
+  }
+  // A row is split over a cluster while that leaves no SM more than three CTAs
+  // and every thread at least two pieces.
   int ctas = 1;
   const int64_t rounds = (static_cast<int64_t>(a.vocab) * sizeof(T) / 16 + kThreads - 1) / kThreads;
-  while (ctas < kMaxCluster && static_cast<int64_t>(a.rows) * ctas * 2 <= device_sm_count() * 4 && rounds > ctas * 2)
+  while (ctas < kMaxCluster && static_cast<int64_t>(a.rows) * ctas * 2 <= device_sm_count() * 3 && rounds > ctas * 2)
     ctas *= 2;
   if (ctas == 1) {
-    logprob_kernel<T, false><<<a.rows, kThreads, 0, s>>>(a, 1);
+    const int grid = std::min(a.rows, device_sm_count() * kRowCtas);
+    logprob_kernel<T, false><<<grid, kThreads + kPostWarps * 32, kRing, s>>>(a, 1);
     return cuda_status(cudaGetLastError());
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * ctas);
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kRing;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -421,6 +654,14 @@ tl_status logprob_launch(const LogprobArgs& a, cudaStream_t s) {
 }
 
 }  // namespace
+
+cudaError_t logprob_read_error(unsigned int* code) {
+  const cudaError_t e = cudaMemcpyFromSymbol(code, g_logprob_error, sizeof(unsigned int));
+  if (e != cudaSuccess || !*code) return e;
+  const unsigned int zero = 0;
+  return cudaMemcpyToSymbol(g_logprob_error, &zero, sizeof(unsigned int));
+}
+
 }  // namespace tl
 
 using namespace tl;

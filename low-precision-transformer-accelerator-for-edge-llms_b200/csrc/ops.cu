@@ -39,6 +39,7 @@ tl_status tl_device_error(void) {
   if (cudaDeviceSynchronize() != cudaSuccess) return TL_ERR_CUDA;
   if (tc_read_error(&code) != cudaSuccess) return TL_ERR_CUDA;
   if (code == 0 && paged_attn_read_error(&code) != cudaSuccess) return TL_ERR_CUDA;
+  if (code == 0 && logprob_read_error(&code) != cudaSuccess) return TL_ERR_CUDA;
   return code ? TL_ERR_TIMEOUT : TL_OK;
 }
 
