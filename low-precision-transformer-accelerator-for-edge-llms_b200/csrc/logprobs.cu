@@ -236,7 +236,7 @@ struct RowSums {
 };
 struct Shared {
   RowSums row[2];
-  Key cand[kCandidates];
+  alignas(16) Key cand[kCandidates];
   Key list[TL_TOP_K_MAX];  // this CTA's largest, in order, then zeros
   Sums total;              // this CTA's sums
   int groups[kThreads];
@@ -304,8 +304,13 @@ TL_DEV void order_candidates(Shared& sh, int n, int k) {
   Post<PT>::sync();
   for (int i = tid; i < n; i += PT) {
     const Key mine = sh.cand[i];
-    int place = 0;
-    for (int j = 0; j < n; ++j) place += sh.cand[j] > mine;
+    int place = 0, j = 0;
+#pragma unroll 4
+    for (; j + 1 < n; j += 2) {
+      const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(sh.cand + j);
+      place += (two.x > mine) + (two.y > mine);
+    }
+    if (j < n) place += sh.cand[j] > mine;
     if (place < k) sh.list[place] = mine;
   }
   Post<PT>::sync();
@@ -410,6 +415,8 @@ __device__ void top_of_share(const Share<T>& w, const RowSums& row, int k, Share
   Post<PT>::sync();
 }
 
+TL_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+TL_DEV void cluster_wait_acquire() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 TL_DEV uint32_t peer_address(const void* p, unsigned rank) {
   uint32_t a;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
@@ -536,12 +543,7 @@ __global__ void __launch_bounds__(CLUSTER ? kThreads : kThreads + kPostWarps * 3
   for (int r = first_row, n = 0; r < a.rows; r += row_step, ++n) {
     const Share<T> w = share(r);
     const int n_tiles = tiles_of(w);
-    int token = -1;
-    float given = 0.0f;
-    if (CLUSTER && tid == 0 && w.rank == 0 && a.tokens) {
-      token = a.tokens[r];
-      if (token >= 0 && token < a.vocab) given = to_f32(w.x[token]);
-    }
+    const int token = CLUSTER && a.tokens ? a.tokens[r] : -1;
     // In ascending order, so that a thread's `at` belongs to the first of equal
     // elements: then an element that beats the bar is in a group that does.
     Running run;
@@ -589,6 +591,7 @@ __global__ void __launch_bounds__(CLUSTER ? kThreads : kThreads + kPostWarps * 3
       __syncwarp();
       if (lane == 0) mbar_arrive(sh.full + (n & 1));
     } else {
+      const float given = token >= 0 && token < a.vocab ? to_f32(w.x[token]) : 0.0f;
       leave(run, a.top_k, sh.row[0]);
       __syncthreads();
       // (every warp joins the warps' sums; lanes beyond them bring nothing)
@@ -605,10 +608,13 @@ __global__ void __launch_bounds__(CLUSTER ? kThreads : kThreads + kPostWarps * 3
           part = {peer_float(&sh.total.m, lane), peer_float(&sh.total.s, lane), peer_float(&sh.total.t, lane)};
         sum = warp_join(part);
         __syncthreads();
-        if (a.top_k) order_candidates<kThreads>(sh, m, a.top_k);
+      }
+      cluster_arrive();  // no CTA goes on while its shared memory may be read
+      if (w.rank == 0) {
+        if (a.top_k) order_candidates<kThreads>(sh, ctas * a.top_k, a.top_k);
         write_row(a, r, tid, sum, sh.list, token, given);
       }
-      cluster_sync();  // no CTA goes on while its shared memory may be read
+      cluster_wait_acquire();
     }
   }
   if (late)  // copies still under way must not land after the CTA has gone
