@@ -40,10 +40,10 @@ namespace tl {
 namespace {
 
 #ifndef VAR_S64
-#define VAR_S64 4
+#define VAR_S64 3
 #endif
 #ifndef VAR_S128
-#define VAR_S128 3
+#define VAR_S128 2
 #endif
 #ifndef VAR_S256
 #define VAR_S256 2
@@ -170,15 +170,16 @@ struct Shape {
   static constexpr int NSUB = RB / SUB;
   static constexpr int KS = D / 16;                     // MMA steps over head_dim
   static constexpr int HALF = KT * RB;                  // bytes of a tile's keys, of its values
-  static constexpr int MERGE = HEADS * D * 4;           // a warp's partial result, in a tile it has read
+  static constexpr int MERGE = HEADS * D * 4;           // a warp's partial result
   static constexpr int STAGE = 2 * HALF;
-  static_assert(MERGE <= STAGE && STAGE % 1024 == 0 && (KT * SUB) % 1024 == 0, "swizzled boxes, partial results");
+  static_assert(STAGE % 1024 == 0 && (KT * SUB) % 1024 == 0, "swizzled boxes");
   static constexpr int STAGES = RB == 64 ? VAR_S64 : RB == 128 ? VAR_S128 : VAR_S256;
-  // shared memory: rings, the query's parts, then scales (int8), tile masks, partial m and l, query scales, barriers
+  // shared memory: rings, the warps' partial results, the query's parts, then scales (int8), tile masks, partial m and l, query scales, barriers
   static constexpr int RING = kWarps * STAGES * STAGE;
   static constexpr int QROW = D * 2;                    // bytes of a query row in 16 bits
   static constexpr int QTILE = 16 * QROW, QTHIRD = PARTS == 3 ? 8 * QROW : 0;
-  static constexpr int QUERY = RING;                    // [m tile]: 16 rows (8 high, 8 low), then 8 third rows
+  static constexpr int PARTS_AT = RING;
+  static constexpr int QUERY = PARTS_AT + kWarps * MERGE;  // [m tile]: 16 rows (8 high, 8 low), then 8 third rows
   static constexpr int SCALES = QUERY + MT * (QTILE + QTHIRD);
   static constexpr int MASKS = SCALES + (I8 ? kWarps * STAGES * 2 * KT * 4 : 0);
   static constexpr int STATS = MASKS + kWarps * STAGES * 4;
@@ -186,6 +187,12 @@ struct Shape {
   static constexpr int BARS = (QSCALE + HEADS * 4 + 7) / 8 * 8;
   static constexpr int SMEM = BARS + kWarps * STAGES * 8 + 1024;  // the base is rounded up to 1024
   static constexpr int UNIT = kWarps * KT;              // positions of one CTA round
+  // What ending an item costs a CTA (its warps' results joined, the next query,
+  // its part written), in rounds: the line leaves such a gap behind every item,
+  // so that CTAs that cross items get fewer rounds. 16 contexts up to 8192
+  // (float16, heads of 128) take 61.3 us with no gap, 54.6, 53.2 and 52.0 with
+  // 1, 2 and 3; 64 up to 2048 over INT8 22.9, 21.1, 21.8, 21.7.
+  static constexpr int GAP = RB == 256 ? 3 : RB == 128 ? 2 : 1;
   static constexpr int RECORD = HEADS * (D + 2);        // floats of a partial result in the workspace
   static constexpr int CTAS = MT == 2 ? 2 : RB == 64 ? VAR_C64 : RB == 128 ? VAR_C128 : VAR_C256;  // CTAs an SM holds
 };
@@ -198,10 +205,10 @@ TL_DEV int row_length(const AttendArgs& a, int r, int* seq) {
   return s < 0 || s >= a.c.n_seqs ? 0 : max(0, min(n, a.c.max_pages * a.c.ps));
 }
 
-// A place in the sequence of units: row r with `units` rounds an item, item
-// `it` of the row (kv head and head block), round `rd` of the item.
+// A place on the line: round `rd` of item `it` (kv head and head block) of row
+// r, whose items have `units` rounds; v is its number on the line.
 struct Place {
-  int r, seq, len, units, it, rd;
+  int r, seq, len, units, it, rd, v;
   template <int UNIT>
   TL_DEV void row(const AttendArgs& a, int row) {
     r = row;
@@ -214,9 +221,11 @@ struct Place {
       ++r;
     }
   }
-  template <int UNIT>
+  template <int UNIT, int GAP>
   TL_DEV void next(const AttendArgs& a, int items) {
+    ++v;
     if (++rd < units) return;
+    v += GAP;
     rd = 0;
     if (++it < items) return;
     it = 0;
@@ -224,7 +233,9 @@ struct Place {
   }
 };
 
-TL_DEV void store_out(void* out, int dt, int64_t i, float4 v) {
+// (a call: the code around the main loop runs once or twice a CTA, from a cold
+// instruction cache, so it is kept short)
+__device__ __noinline__ void store_out(void* out, int dt, int64_t i, float4 v) {
   if (dt == TL_F32) {
     *reinterpret_cast<float4*>(static_cast<float*>(out) + i) = v;
   } else if (dt == TL_BF16) {
@@ -237,20 +248,6 @@ TL_DEV void store_out(void* out, int dt, int64_t i, float4 v) {
         make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
   }
 }
-TL_DEV float4 load_act4(const void* p, int dt, int64_t i) {
-  if (dt == TL_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-  const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-  float2 x, y;
-  if (dt == TL_BF16) {
-    x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x));
-    y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
-  } else {
-    x = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
-    y = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-  }
-  return make_float4(x.x, x.y, y.x, y.y);
-}
-
 // Rows without positions are on nobody's line: zeros and -infinity.
 template <int D>
 TL_DEV void zero_empty_rows(const AttendArgs& a) {
@@ -262,6 +259,114 @@ TL_DEV void zero_empty_rows(const AttendArgs& a) {
       store_out(a.out, a.q_dtype, base * D + i, make_float4(0, 0, 0, 0));
     if (a.lse)
       for (int i = threadIdx.x; i < a.heads; i += kWarps * 32) a.lse[base + i] = -INFINITY;
+  }
+}
+
+// Joins the parts of an item, x = (first CTA, last CTA, first row of out, heads).
+template <typename S>
+__device__ void join_records(const AttendArgs& a, unsigned char* smem, int4 x) {
+  constexpr int D = S::D;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int c0 = x.x, c1 = x.y, nh = x.w;
+  const int64_t head0 = x.z;
+  // Of each batch of records, a warp a head turns the maxima and sums into
+  // weights in shared memory, and every thread sums its columns. It runs after
+  // all other work of the item, so its few rounds of L2 latency show: as many
+  // loads as registers allow are in flight, the first ones before the weights
+  // are known (37 records of 8 x 128: {T_JOIN}).
+  constexpr int COLS = S::HEADS * D / (kWarps * 128), BATCH = 64, DEPTH = (S::CTAS > 2 ? 16 : 32) / COLS;
+  float* weight = reinterpret_cast<float*>(smem + S::PARTS_AT);  // [head][record]
+  float* top = reinterpret_cast<float*>(smem + S::STATS);        // [head]: maximum, sum, factor of the old sums
+  float* sum = top + S::HEADS;
+  float* old = sum + S::HEADS;
+  auto record = [&](int b) { return a.records + (static_cast<int64_t>(b) * 2 + (b == c0)) * S::RECORD; };
+  float4 v[COLS], y[DEPTH][COLS];
+  auto load = [&](int b, int end) {
+#pragma unroll
+    for (int k = 0; k < DEPTH; ++k)
+#pragma unroll
+      for (int c = 0; c < COLS; ++c)  // (past the end: the last one again)
+        y[k][c] = __ldcg(reinterpret_cast<const float4*>(record(min(b + k, end - 1)) + tid * 4 + c * kWarps * 128));
+  };
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) v[c] = make_float4(0, 0, 0, 0);
+  __syncthreads();
+  if (tid < S::HEADS) {
+    top[tid] = -INFINITY;
+    sum[tid] = 0.0f;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int b0 = c0; b0 <= c1; b0 += BATCH) {
+    const int end = min(b0 + BATCH, c1 + 1);
+    // lane = records b0 + lane, + 32; warp w takes heads w, w + 4, ...
+    float rm[S::HEADS / kWarps][2], rl[S::HEADS / kWarps][2];
+#pragma unroll
+    for (int k = 0; k < S::HEADS / kWarps; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float* p = record(min(b0 + lane + 32 * i, end - 1)) + S::HEADS * D + warp + kWarps * k;
+        rm[k][i] = __ldcg(p);
+        rl[k][i] = __ldcg(p + S::HEADS);
+      }
+    load(b0, end);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (b0 + lane + 32 * i >= end)
+#pragma unroll
+        for (int k = 0; k < S::HEADS / kWarps; ++k) rm[k][i] = -INFINITY, rl[k][i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < S::HEADS / kWarps; ++k) {
+      const int h = warp + kWarps * k;
+      const float m0 = top[h], m1 = fmaxf(m0, warp_max(fmaxf(rm[k][0], rm[k][1])));
+      float l1 = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float e = rm[k][i] == -INFINITY ? 0.0f : exp2_approx(rm[k][i] - m1);
+        weight[h * BATCH + lane + 32 * i] = e;
+        l1 += e * rl[k][i];
+      }
+      l1 = warp_sum(l1);
+      if (lane == 0) {
+        const float f = m0 == -INFINITY ? 0.0f : exp2_approx(m0 - m1);
+        top[h] = m1;
+        sum[h] = sum[h] * f + l1;
+        old[h] = f;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) {
+      const float f = old[(tid * 4 + c * kWarps * 128) / D];
+      v[c].x *= f, v[c].y *= f, v[c].z *= f, v[c].w *= f;
+    }
+#pragma unroll 1
+    for (int b1 = b0; b1 < end; b1 += DEPTH) {
+      if (b1 > b0) load(b1, end);
+#pragma unroll
+      for (int k = 0; k < DEPTH; ++k)
+        if (b1 + k < end) {
+#pragma unroll
+          for (int c = 0; c < COLS; ++c) {
+            const float e = weight[(tid * 4 + c * kWarps * 128) / D * BATCH + b1 + k - b0];
+            v[c].x += y[k][c].x * e;
+            v[c].y += y[k][c].y * e;
+            v[c].z += y[k][c].z * e;
+            v[c].w += y[k][c].w * e;
+          }
+        }
+    }
+    __syncthreads();  // the weights have been used
+  }
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) {
+    const int h = (tid * 4 + c * kWarps * 128) / D, d = (tid * 4) % D;
+    if (h >= nh) continue;
+    const bool empty = top[h] == -INFINITY && sum[h] == 0.0f;
+    const float inv = empty ? 0.0f : 1.0f / sum[h];
+    store_out(a.out, a.q_dtype, (head0 + h) * D + d,
+              make_float4(v[c].x * inv, v[c].y * inv, v[c].z * inv, v[c].w * inv));
+    if (a.lse && d == 0) a.lse[head0 + h] = empty ? -INFINITY : (top[h] + log2f(sum[h])) * kLn2;
   }
 }
 
@@ -281,7 +386,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   __shared__ int sh_units[kWarps];
   __shared__ int4 sh_first;  // the stretch's first row, the units before it, the row's sequence and length
-  __shared__ int sh_last;
+  __shared__ int sh_last[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int items = a.c.hkv * a.blocks;
 
@@ -298,7 +403,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
   bool empty_row = false;  // a row without positions that this CTA writes
   for (int r = r0; r < r1; ++r) {
     len = row_length(a, r, &seq);
-    mine += (len + UNIT - 1) / UNIT;
+    mine += len ? (len + UNIT - 1) / UNIT + S::GAP : 0;
     if (len == 0) empty_row |= r % ctas == cta;
   }
   mine *= items;
@@ -327,39 +432,68 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
     int r = r0;
     for (; per > 1; ++r) {
       len = row_length(a, r, &seq);
-      const int n = (len + UNIT - 1) / UNIT * items;
+      const int n = len ? ((len + UNIT - 1) / UNIT + S::GAP) * items : 0;
       if (u0 < before + n) break;
       before += n;
     }
     sh_first = make_int4(r, before, seq, len);
   }
   __syncthreads();
-  const int n_units = u1 - u0;
   Place use;
   use.r = sh_first.x;
   use.seq = sh_first.z;
   use.len = sh_first.w;
   use.units = (use.len + UNIT - 1) / UNIT;
-  use.it = (u0 - sh_first.y) / use.units;
-  use.rd = (u0 - sh_first.y) - use.it * use.units;
+  use.it = (u0 - sh_first.y) / (use.units + S::GAP);
+  use.rd = (u0 - sh_first.y) - use.it * (use.units + S::GAP);
+  use.v = u0;
+  if (use.rd >= use.units) {  // in a gap
+    use.v += use.units + S::GAP - use.rd - 1;
+    use.v -= S::GAP;
+    use.rd = use.units - 1;
+    use.next<UNIT, S::GAP>(a, items);
+  }
+  if (use.v >= u1) {
+    if (empty_row) zero_empty_rows<D>(a);
+    return;
+  }
   Place fill = use;
 
   // The query of the item at `p`: kQ consecutive elements a thread, first as
   // loaded, then as 16-bit parts in shared memory.
   constexpr int kQ = S::HEADS * D / (kWarps * 32), kLanes = D / kQ;  // elements of a thread, threads of a head
   const int qh = tid / kLanes, qd = tid % kLanes * kQ;
-  float x[kQ];
+  uint4 raw[kQ / 4];
   auto load_query = [&](const Place& p) {
     const int kvh = p.it / a.blocks, hb = p.it - kvh * a.blocks;
     const bool live = hb * S::HEADS + qh < a.group;
     const int64_t base = p.r * a.ldq + static_cast<int64_t>(kvh * a.group + (live ? hb * S::HEADS + qh : 0)) * D + qd;
+    const char* q = static_cast<const char*>(a.q) + base * (a.q_dtype == TL_F32 ? 4 : 2);
 #pragma unroll
-    for (int e = 0; e < kQ; e += 4) {
-      const float4 y = live ? load_act4(a.q, a.q_dtype, base + e) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      x[e] = y.x, x[e + 1] = y.y, x[e + 2] = y.z, x[e + 3] = y.w;
+    for (int e = 0; e < kQ / 4; ++e) raw[e] = make_uint4(0, 0, 0, 0);
+    if (!live) return;
+    if (a.q_dtype == TL_F32) {
+#pragma unroll
+      for (int e = 0; e < kQ / 4; ++e) raw[e] = *reinterpret_cast<const uint4*>(q + 16 * e);
+    } else if constexpr (kQ == 4) {
+      const uint2 y = *reinterpret_cast<const uint2*>(q);
+      raw[0].x = y.x;
+      raw[0].y = y.y;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kQ / 8; ++e) raw[e] = *reinterpret_cast<const uint4*>(q + 16 * e);
     }
   };
   auto store_query = [&]() {
+    float x[kQ];
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(raw);
+#pragma unroll
+    for (int e = 0; e < kQ; ++e) {
+      const uint32_t half = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
+      x[e] = a.q_dtype == TL_F32    ? __uint_as_float(w[e])
+             : a.q_dtype == TL_BF16 ? __uint_as_float(half << 16)
+                                    : __half2float(__ushort_as_half(static_cast<unsigned short>(half)));
+    }
     float f = 1.0f, back = a.scale * kLog2e;
     if constexpr (!S::BF) {
       // a power of two that takes the row's largest element to [2^10, 2^11)
@@ -451,30 +585,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
       }
     }
   };
-  // the first tiles' pages are looked up together, then their copies start
-  int filled = 0, next_row = -1;
-  {
-    int rows[S::STAGES];
-#pragma unroll
-    for (int i = 0; i < S::STAGES; ++i) {
-      rows[i] = -1;
-      if (i < n_units) {
-        rows[i] = lookup(fill);
-        if (i < S::STAGES - 1) fill.next<UNIT>(a, items);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < S::STAGES - 1; ++i) {
-      if (filled < n_units) {
-        copy_tile(i, rows[i]);
-        ++filled;
-      }
-      if constexpr (S::I8) cp_async_commit();
-    }
-    next_row = rows[S::STAGES - 1];
-  }
-  store_query();
-  __syncthreads();
+  int filled = 0, next_row = lookup(fill);
 
   // Byte offsets of this lane's ldmatrix rows, swizzled: 16-byte piece c of row
   // r of a box lies at piece c ^ (r % 8) of 128-byte rows, c ^ (r / 2 % 4) of
@@ -492,10 +603,16 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
   float m[MT], l[MT];
   float vu = 0.0f, vinv = 1.0f;  // int8: the power of two that value scales are divided by, its inverse
   bool fresh = true;
+  int pending = 0;  // items that other CTAs have parts of: at most the stretch's first and last
+  int4 late0{}, late1{};
 
-  for (int i = 0, stage = 0, phase = 0; i < n_units; ++i) {
+  // The first STAGES turns only fill the ring.
+  for (int i = -S::STAGES, stage = 0, phase = 1; i < 0 || use.v < u1; ++i) {
+    if (i >= 0) {
     if (fresh) {
       fresh = false;
+      store_query();
+      __syncthreads();  // the query is there, the last item's partial results have been read
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         qscale[mt] = reinterpret_cast<const float*>(smem + S::QSCALE)[mt * 8 + g];
@@ -511,23 +628,14 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
     }
 
     if (late ? !mbar_try_wait(bars + stage, phase) : !mbar_wait_err(bars + stage, phase, 1u, &g_paged_error)) late = true;
-    if constexpr (S::I8) cp_async_wait<S::STAGES - 2>();
+    if constexpr (S::I8) cp_async_wait<S::STAGES - 1>();
     __syncwarp();
-    // refill the stage consumed one round ago
-    if (filled < n_units) {
-      copy_tile(stage == 0 ? S::STAGES - 1 : stage - 1, next_row);
-      fill.next<UNIT>(a, items);
-      ++filled;
-      next_row = filled < n_units ? lookup(fill) : -1;
-    }
-    if constexpr (S::I8) cp_async_commit();
-
     const uint32_t kbase = ring32 + stage * S::STAGE, vbase = kbase + S::HALF;
     const float* sc = scales + stage * 2 * KT;
     const unsigned live = masks[stage];
+    constexpr unsigned full = KT == 32 ? 0xffffffffu : 0xffffu;
     if constexpr (!S::I8) {
       // values of positions that do not exist must not meet a probability of zero as a NaN
-      constexpr unsigned full = KT == 32 ? 0xffffffffu : 0xffffu;
       if (live != 0 && live != full) {
         for (int r = 0; r < KT; ++r)
           if (!(live >> r & 1) && lane < S::RB / 16)
@@ -593,7 +701,6 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
         if constexpr (S::I8) {
           kscale = *reinterpret_cast<const float2*>(sc + 8 * j + 2 * t);
         }
-        const bool in0 = live >> (8 * j + 2 * t) & 1, in1 = live >> (8 * j + 2 * t + 1) & 1;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           float x = (c[j][mt][0] + c[j][mt][2]) * qscale[mt], y = (c[j][mt][1] + c[j][mt][3]) * qscale[mt];
@@ -601,10 +708,18 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
             x *= kscale.x;
             y *= kscale.y;
           }
-          s[mt][j][0] = in0 ? x : -INFINITY;
-          s[mt][j][1] = in1 ? y : -INFINITY;
+          s[mt][j][0] = x;
+          s[mt][j][1] = y;
         }
       }
+      if (live != full)
+#pragma unroll
+        for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (!(live >> (8 * j + 2 * t + e) & 1))
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) s[mt][j][e] = -INFINITY;
       // ---- running reference
       float vs[KT / 8][2];
       float vtop = 0.0f;
@@ -708,11 +823,22 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
         }
     }
 
+    }
+
+    // ---- the tile has been read by all lanes: the next one for its place
+    __syncwarp();
+    if (fill.v < u1) {
+      copy_tile(stage, next_row);
+      ++filled;
+      fill.next<UNIT, S::GAP>(a, items);
+      next_row = fill.v < u1 ? lookup(fill) : -1;
+    }
+    if constexpr (S::I8) cp_async_commit();
+
     // ---- the item's (or the stretch's) last round: join the warps
-    if (use.rd + 1 == use.units || i + 1 == n_units) {
-      float* part = reinterpret_cast<float*>(ring + stage * S::STAGE);
+    if (i >= 0 && (use.rd + 1 == use.units || use.v + 1 == u1)) {
+      float* part = reinterpret_cast<float*>(smem + S::PARTS_AT + warp * S::MERGE);
       float* stats = reinterpret_cast<float*>(smem + S::STATS);  // [warp][m, l][head]
-      __syncwarp();  // the stage's tile has been read by all lanes
       const float vback = S::I8 ? vu : 1.0f;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -743,16 +869,17 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
       }
       // the next item's query arrives while this one is joined
       const Place done = use;
-      use.next<UNIT>(a, items);
-      if (i + 1 < n_units) load_query(use);
+      use.next<UNIT, S::GAP>(a, items);
+      if (use.v < u1) load_query(use);
       __syncthreads();
       const int kvh = done.it / a.blocks, hb = done.it - kvh * a.blocks;
       const int nh = min(S::HEADS, a.group - hb * S::HEADS);
-      const int first = u0 + i - done.rd;  // the item's first unit on the line
+      const int first = done.v - done.rd;  // the item's first round on the line
       const int c0 = first / chunk, c1 = (first + done.units - 1) / chunk;
       const bool whole = c0 == c1;
       const int64_t head0 = static_cast<int64_t>(done.r) * a.heads + kvh * a.group + hb * S::HEADS;
       float* rec = a.records + (static_cast<int64_t>(cta) * 2 + (cta == c0)) * S::RECORD;
+#pragma unroll 1
       for (int x = tid * 4; x < (whole ? nh : S::HEADS) * D; x += kWarps * 128) {
         const int h = x / D, d = x % D;
         float M = -INFINITY, L = 0.0f, pm[kWarps];
@@ -764,7 +891,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
         }
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float* p = reinterpret_cast<const float*>(smem + (w * S::STAGES + stage) * S::STAGE);
+          const float* p = reinterpret_cast<const float*>(smem + S::PARTS_AT + w * S::MERGE);
           const float f = pm[w] == -INFINITY ? 0.0f : exp2_approx(pm[w] - M);
           const float4 y = *reinterpret_cast<const float4*>(p + h * D + (d ^ (8 * (h & 7))));
           L += f * stats[(w * 2 + 1) * S::HEADS + h];
@@ -787,117 +914,41 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
         }
       }
       if (!whole) {
-        __threadfence();
-        __syncthreads();
-        if (tid == 0) {
-          const unsigned n = atomicAdd(a.tickets + c0, 1u);
-          sh_last = n == static_cast<unsigned>(c1 - c0);
-          if (sh_last) a.tickets[c0] = 0;
-        }
-        __syncthreads();
-        if (sh_last) {
-          __threadfence();
-          // A batch's maxima and sums go to shared memory, a warp a head turns
-          // them into weights, then every thread sums its columns.
-          constexpr int COLS = S::HEADS * D / (kWarps * 128), BATCH = 32, DEPTH = 16 / COLS;
-          float* bm = reinterpret_cast<float*>(smem + stage * S::STAGE);  // [head][record]: weights
-          float* top = reinterpret_cast<float*>(smem + S::STATS);  // [head]: maximum, sum, factor of the old sums
-          float* sum = top + S::HEADS;
-          float* old = sum + S::HEADS;
-          float4 v[COLS];
-#pragma unroll
-          for (int c = 0; c < COLS; ++c) v[c] = make_float4(0, 0, 0, 0);
-          __syncthreads();
-          if (tid < S::HEADS) {
-            top[tid] = -INFINITY;
-            sum[tid] = 0.0f;
-          }
-          for (int b0 = c0; b0 <= c1; b0 += BATCH) {
-            const int n = min(BATCH, c1 + 1 - b0);
-            // lane = record, warp w takes heads w, w + 4, ...
-            float rm[S::HEADS / kWarps], rl[S::HEADS / kWarps];
-#pragma unroll
-            for (int k = 0; k < S::HEADS / kWarps; ++k) {
-              const int b = b0 + min(lane, n - 1);
-              const float* p = a.records + (static_cast<int64_t>(b) * 2 + (b == c0)) * S::RECORD + S::HEADS * D +
-                               warp + kWarps * k;
-              rm[k] = __ldcg(p);
-              rl[k] = __ldcg(p + S::HEADS);
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < S::HEADS / kWarps; ++k) {
-              const int h = warp + kWarps * k;
-              const float m0 = top[h], m1 = fmaxf(m0, warp_max(rm[k]));
-              const float e = lane >= n || rm[k] == -INFINITY ? 0.0f : exp2_approx(rm[k] - m1);
-              const float l1 = warp_sum(lane < n ? e * rl[k] : 0.0f);
-              bm[h * BATCH + lane] = e;
-              if (lane == 0) {
-                const float f = m0 == -INFINITY ? 0.0f : exp2_approx(m0 - m1);
-                top[h] = m1;
-                sum[h] = sum[h] * f + l1;
-                old[h] = f;
-              }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int c = 0; c < COLS; ++c) {
-              const float f = old[(tid * 4 + c * kWarps * 128) / D];
-              v[c].x *= f, v[c].y *= f, v[c].z *= f, v[c].w *= f;
-            }
-            for (int b1 = 0; b1 < n; b1 += DEPTH) {
-              float4 y[DEPTH][COLS];
-#pragma unroll
-              for (int k = 0; k < DEPTH; ++k) {
-                const int b = b0 + min(b1 + k, n - 1);
-                const float* p = a.records + (static_cast<int64_t>(b) * 2 + (b == c0)) * S::RECORD + tid * 4;
-#pragma unroll
-                for (int c = 0; c < COLS; ++c)
-                  y[k][c] = __ldcg(reinterpret_cast<const float4*>(p + c * kWarps * 128));
-              }
-#pragma unroll
-              for (int k = 0; k < DEPTH; ++k)
-                if (b1 + k < n) {
-#pragma unroll
-                  for (int c = 0; c < COLS; ++c) {
-                    const float e = bm[(tid * 4 + c * kWarps * 128) / D * BATCH + b1 + k];
-                    v[c].x += y[k][c].x * e;
-                    v[c].y += y[k][c].y * e;
-                    v[c].z += y[k][c].z * e;
-                    v[c].w += y[k][c].w * e;
-                  }
-                }
-            }
-          }
-#pragma unroll
-          for (int c = 0; c < COLS; ++c) {
-            const int h = (tid * 4 + c * kWarps * 128) / D, d = (tid * 4) % D;
-            if (h >= nh) continue;
-            const bool empty = top[h] == -INFINITY && sum[h] == 0.0f;
-            const float inv = empty ? 0.0f : 1.0f / sum[h];
-            store_out(a.out, a.q_dtype, (head0 + h) * D + d,
-                      make_float4(v[c].x * inv, v[c].y * inv, v[c].z * inv, v[c].w * inv));
-            if (a.lse && d == 0) a.lse[head0 + h] = empty ? -INFINITY : (top[h] + log2f(sum[h])) * kLn2;
-          }
-        }
+        if (pending == 0)
+          late0 = make_int4(c0, c1, static_cast<int>(head0), nh);
+        else
+          late1 = make_int4(c0, c1, static_cast<int>(head0), nh);
+        ++pending;
       }
-      if (i + 1 < n_units) store_query();
-      fence_proxy_async_smem();
-      __syncthreads();  // the stages that held the partial results may be refilled
       fresh = true;
-    } else {
-      use.next<UNIT>(a, items);
+    } else if (i >= 0) {
+      use.next<UNIT, S::GAP>(a, items);
     }
     if (++stage == S::STAGES) {
       stage = 0;
       phase ^= 1;
     }
   }
-  if (late)  // copies still under way must not land after the CTA has gone
-    for (int s = 0; s < S::STAGES && s < n_units; ++s) {
-      const int uses = (n_units - 1 - s) / S::STAGES;
-      mbar_wait_err(bars + s, uses & 1, 2u, &g_paged_error);
+  if (pending) {
+    // tickets are drawn at the end, when all parts are written: the CTA that
+    // draws an item's last one joins its parts
+    __threadfence();
+    __syncthreads();
+    if (tid < pending) {
+      const int4 x = tid ? late1 : late0;
+      const bool last = atomicAdd(a.tickets + x.x, 1u) == static_cast<unsigned>(x.y - x.x);
+      if (last) a.tickets[x.x] = 0;
+      sh_last[tid] = last;
     }
+    __syncthreads();
+    __threadfence();
+#pragma unroll 1
+    for (int j = 0; j < pending; ++j)
+      if (sh_last[j]) join_records<S>(a, smem, j ? late1 : late0);
+  }
+  if (late)  // copies still under way must not land after the CTA has gone
+    for (int i = max(0, filled - S::STAGES); i < filled; ++i)
+      mbar_wait_err(bars + i % S::STAGES, i / S::STAGES & 1, 2u, &g_paged_error);
   if (empty_row) zero_empty_rows<D>(a);
 }
 
@@ -906,7 +957,7 @@ tl_status attend_launch(AttendArgs& a, cudaStream_t s) {
   // the line of units has 31 bits
   const int64_t most = static_cast<int64_t>(a.c.hkv) * a.blocks *
                        ((static_cast<int64_t>(a.c.max_pages) * a.c.ps + S::UNIT - 1) / S::UNIT);
-  if (most > INT32_MAX / a.rows) return TL_ERR_OUT_OF_RANGE;
+  if (most + static_cast<int64_t>(a.c.hkv) * a.blocks * S::GAP > INT32_MAX / a.rows) return TL_ERR_OUT_OF_RANGE;
   // once a device: the ring needs more shared memory than the default limit
   static bool ready[64];
   int dev = 0;
@@ -983,7 +1034,7 @@ tl_status tl_paged_attn_decode(const tl_paged_kv* cache, const tl_paged_attn_arg
   if (!aligned_to(x.q, 16) || !aligned_to(x.out, 16) || !aligned_to(x.workspace, 16)) return TL_ERR_INVALID_ARGUMENT;
   if (x.workspace_bytes < tl_paged_attn_workspace_bytes(x.heads, cache->kv_heads, cache->head_dim))
     return TL_ERR_OUT_OF_RANGE;
-  if (!x.seq && x.rows > x.n_seqs) return TL_ERR_OUT_OF_RANGE;
+  if ((!x.seq && x.rows > x.n_seqs) || x.rows > INT32_MAX / x.heads) return TL_ERR_OUT_OF_RANGE;
   a.q = x.q;
   a.ldq = x.q_stride;
   a.q_dtype = x.q_dtype;
