@@ -9,7 +9,8 @@
 // t = sum f (t_i + e s_i) with e = (m_i - m) log2 e, f = 2^e.
 //
 // The k largest. Every thread remembers the largest of its elements while it
-// sums; a thread's elements are a group. The k-th largest of the groups'
+// sums (for long lists afresh in each of four parts of the row); the elements
+// of a thread and part are a group. The k-th largest of the groups'
 // maxima is no larger than the k-th largest element, so only groups whose
 // maximum reaches it can hold one of the k, and only their elements (read
 // again, from L2) are compared: the single pass over the row does no work for
@@ -47,7 +48,7 @@ constexpr int kPostWarps = 2;
 constexpr int kRowCtas = 3;
 constexpr int kCandidates = 512;
 constexpr int kMaxCluster = 8;
-constexpr int kPicks = TL_TOP_K_MAX / kWarps + 1;  // largest maxima taken of a warp
+constexpr int kParts = 4;
 constexpr int kRing = kWarps * kStages * kTileBytes;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -136,6 +137,10 @@ struct Chunk {
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
                  : "l"(p));
+  }
+  TL_DEV void clear() {  // minus infinity
+    const uint32_t x = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __nv_bfloat16>::value ? 0xff80ff80u : 0xfc00fc00u;
+    w = make_uint4(x, x, x, x);
   }
   TL_DEV void load_shared(const unsigned char* p) { w = *reinterpret_cast<const uint4*>(p); }
   TL_DEV void get(float* x) const {
@@ -231,15 +236,15 @@ struct Running {
 // What the summing warps leave of a row.
 struct RowSums {
   Sums sums[kWarps];
-  Key picks[kWarps * kPicks];  // of each warp, its largest groups' maxima
-  Key best[kThreads];          // every group's maximum
+  Key picks[TL_TOP_K_MAX + 2 * kWarps];  // of each warp with tiles, its lanes' largest maxima
+  Key best[kParts][kThreads];            // every group's maximum
 };
 struct Shared {
   RowSums row[2];
   alignas(16) Key cand[kCandidates];
   Key list[TL_TOP_K_MAX];  // this CTA's largest, in order, then zeros
   Sums total;              // this CTA's sums
-  int groups[kThreads];
+  int groups[kParts * kThreads];
   int n_groups, n_cand;
   Key reduce[kWarps];
   uint64_t tiles[kWarps * kStages], full[2], empty[2];  // barriers
@@ -253,11 +258,17 @@ template <typename T>
 struct Share {
   static constexpr int N = Chunk<T>::N;
   const T* x;
-  int vocab, head, chunks, ctas, rank;
+  int vocab, head, chunks, ctas, rank, parts;
   TL_DEV int chunk_first(int i) const { return head + i * N; }
   TL_DEV int tiles() const { return (chunks + kTile - 1) / kTile; }
   TL_DEV int tile(int warp, int i) const { return rank * kWarps + warp + i * step(); }  // warp's i-th tile
   TL_DEV int step() const { return ctas * kWarps; }
+  TL_DEV int turns() const { return (tiles() + step() - 1) / step(); }          // the most tiles of a warp
+  TL_DEV int part_turns() const { return max(1, (turns() + parts - 1) / parts); }
+  // the CTA's warps that have tiles (at least one: the loose elements' warp), and the maxima each picks, so that
+  // together they pick k + 1 at least
+  TL_DEV int busy() const { return max(1, min(kWarps, tiles() - rank * kWarps)); }
+  TL_DEV int picks(int k) const { return min(32, (k + busy() - 1) / busy() + 1); }
   // the loose element of a thread, -1: none
   TL_DEV int loose(int thread) const {
     if (rank) return -1;
@@ -278,19 +289,17 @@ struct Post {
   }
 };
 
-// A warp's part of what is left of a row.
-TL_DEV void leave(const Running& run, int top_k, RowSums& row) {
+// A warp's part of what is left of a row; `most`: the lane's largest maximum.
+template <typename T>
+TL_DEV void leave(const Share<T>& w, const Running& run, Key most, int top_k, RowSums& row) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Sums sum = warp_join(run.sums());
   if (lane == 0) row.sums[warp] = sum;
-  if (!top_k) return;
-  const Key mine = run.best > -INFINITY ? argmax_key(run.best + 0.0f, run.at) : 0;
-  row.best[threadIdx.x] = mine;
-  const int picks = (top_k + kWarps - 1) / kWarps + 1;
-  Key left = mine;
+  if (!top_k || warp >= w.busy()) return;
+  const int picks = w.picks(top_k);
   for (int i = 0; i < picks; ++i) {
-    const Key top = warp_max_key(left);
-    if (left == top) left = 0;  // keys of two lanes differ unless both are empty
+    const Key top = warp_max_key(most);
+    if (most == top) most = 0;  // keys of two lanes differ unless both are empty
     if (lane == 0) row.picks[warp * picks + i] = top;
   }
 }
@@ -321,7 +330,7 @@ template <typename T, int PT>
 __device__ void top_of_share(const Share<T>& w, const RowSums& row, int k, Shared& sh) {
   constexpr int N = Chunk<T>::N, PW = PT / 32;
   const int tid = Post<PT>::tid(), lane = tid & 31, warp = tid >> 5;
-  const int n_picks = kWarps * ((k + kWarps - 1) / kWarps + 1);
+  const int n_picks = w.busy() * w.picks(k);
   if (tid == 0) sh.n_groups = sh.n_cand = 0;
   // the k-th largest of the picks (0 if there are fewer)
   Key bar = ~0ull;
@@ -333,8 +342,11 @@ __device__ void top_of_share(const Share<T>& w, const RowSums& row, int k, Share
   }
   bar = ~warp_max_key(~bar);
   Post<PT>::sync();
-  for (int g = tid; g < kThreads; g += PT)
-    if (row.best[g] && row.best[g] >= bar) sh.groups[atomicAdd(&sh.n_groups, 1)] = g;
+  const int parts = (w.turns() + w.part_turns() - 1) / w.part_turns();
+  for (int g = tid; g < max(1, parts) * kThreads; g += PT) {
+    const Key best = row.best[g / kThreads][g % kThreads];
+    if (best && best >= bar) sh.groups[atomicAdd(&sh.n_groups, 1)] = g;
+  }
   Post<PT>::sync();
   const int n_groups = sh.n_groups;
   const float bar_value = bar ? key_value(bar) : -INFINITY;
@@ -346,7 +358,7 @@ __device__ void top_of_share(const Share<T>& w, const RowSums& row, int k, Share
     if (at < kCandidates) sh.cand[at] = key;
   };
   // the groups' pieces, spread over the threads, a few loads in flight
-  const int per = (w.tiles() + w.step() - 1) / w.step() * kUnroll, pieces = n_groups * per;
+  const int per = w.part_turns() * kUnroll, pieces = n_groups * per;
   constexpr int F = PT == kThreads ? 1 : 4;
   for (int i0 = tid; i0 < pieces; i0 += PT * F) {
     Chunk<T> y[F];
@@ -356,8 +368,8 @@ __device__ void top_of_share(const Share<T>& w, const RowSums& row, int k, Share
       const int i = i0 + f * PT;
       c[f] = w.chunks;
       if (i < pieces) {
-        const int g = sh.groups[i / per], place = i % per;
-        c[f] = w.tile(g >> 5, place / kUnroll) * kTile + place % kUnroll * 32 + (g & 31);
+        const int g = sh.groups[i / per], place = i % per, turn = g / kThreads * w.part_turns() + place / kUnroll;
+        c[f] = w.tile(g % kThreads >> 5, turn) * kTile + place % kUnroll * 32 + (g & 31);
       }
       if (c[f] < w.chunks) y[f].load(w.x + w.chunk_first(c[f]));
     }
@@ -370,8 +382,9 @@ __device__ void top_of_share(const Share<T>& w, const RowSums& row, int k, Share
         for (int e = 0; e < N; ++e) offer(v[e], w.chunk_first(c[f]) + e);
       }
   }
-  for (int i = tid; i < n_groups; i += PT)
-    if (const int loose = w.loose(sh.groups[i]); loose >= 0) offer(to_f32(w.x[loose]), loose);
+  // (the loose elements are few, and in groups of several parts: all are compared)
+  if (tid < 2 * N)
+    if (const int loose = w.loose(tid); loose >= 0) offer(to_f32(w.x[loose]), loose);
   Post<PT>::sync();
   const int n = sh.n_cand;
   if (n <= kCandidates) {
@@ -473,14 +486,13 @@ __global__ void __launch_bounds__(CLUSTER ? kThreads : kThreads + kPostWarps * 3
     w.chunks = (a.vocab - w.head) / N;
     w.ctas = CLUSTER ? ctas : 1;
     w.rank = CLUSTER ? blockIdx.x % ctas : 0;
+    w.parts = a.top_k > 8 ? kParts : 1;
     return w;
-  };
-  auto tiles_of = [&](const Share<T>& w) {
-    return w.tile(warp, 0) < w.tiles() ? (w.tiles() - 1 - w.tile(warp, 0)) / w.step() + 1 : 0;
   };
   bool late = false;  // a wait has run out: the results are void, the host learns of it
   auto wait = [&](uint64_t* bar, int parity, unsigned code) {
-    if (late ? !mbar_try_wait(bar, parity) : !mbar_wait_err(bar, parity, code, &g_logprob_error)) late = true;
+    if (mbar_try_wait(bar, parity)) return;  // (the clock is read only if there is something to wait for)
+    if (late || !mbar_wait_err(bar, parity, code, &g_logprob_error)) late = true;
   };
   if (!CLUSTER && tid == 0)
     for (int i = 0; i < 2; ++i) {
@@ -516,83 +528,100 @@ __global__ void __launch_bounds__(CLUSTER ? kThreads : kThreads + kPostWarps * 3
 
   // ---- the warp's ring, filled kStages tiles ahead, also across rows
   unsigned char* ring = rings + warp * kStages * kTileBytes;
-  int fill_row = first_row, fill_i = 0, filled = 0;
-  Share<T> fill_w = share(fill_row);
-  int fill_n = tiles_of(fill_w);
+  // (addresses and sizes move by a constant from tile to tile)
+  const int step_bytes = (CLUSTER ? ctas : 1) * kWarps * kTileBytes;
+  int fill_row = first_row, fill_left = 0, filled = 0;  // bytes of the row from the next tile on
+  const char* fill_at = nullptr;
+  auto fill_start = [&]() {
+    const Share<T> w = share(fill_row);
+    const int first = w.tile(warp, 0) * kTile;
+    fill_at = reinterpret_cast<const char*>(w.x + w.head) + first * 16ll;
+    fill_left = (w.chunks - first) * 16;
+  };
   auto fill = [&](int stage) {
-    while (fill_i >= fill_n) {
+    while (fill_left <= 0) {
       fill_row += row_step;
       if (fill_row >= a.rows) return;
-      fill_w = share(fill_row);
-      fill_n = tiles_of(fill_w);
-      fill_i = 0;
+      fill_start();
     }
     if (lane == 0) {
-      const int first = fill_w.tile(warp, fill_i) * kTile;
-      const uint32_t bytes = min(kTile, fill_w.chunks - first) * 16;
+      const uint32_t bytes = min(fill_left, kTileBytes);
       mbar_arrive_expect_tx(bars + stage, bytes);
-      bulk_load(ring + stage * kTileBytes, fill_w.x + fill_w.chunk_first(first), bytes, bars + stage);
+      bulk_load(ring + stage * kTileBytes, fill_at, bytes, bars + stage);
     }
-    ++fill_i;
+    fill_at += step_bytes;
+    fill_left -= step_bytes;
     ++filled;
   };
+  fill_start();
   for (int i = 0; i < kStages; ++i)
     if (fill_row < a.rows) fill(i);
 
   int stage = 0, phase = 0;
   for (int r = first_row, n = 0; r < a.rows; r += row_step, ++n) {
     const Share<T> w = share(r);
-    const int n_tiles = tiles_of(w);
     const int token = CLUSTER && a.tokens ? a.tokens[r] : -1;
     // In ascending order, so that a thread's `at` belongs to the first of equal
     // elements: then an element that beats the bar is in a group that does.
     Running run;
-    const int loose = w.loose(tid);
+    Key most = 0;
+    RowSums& left = sh.row[CLUSTER ? 0 : n & 1];
+    if constexpr (!CLUSTER) wait(sh.empty + (n & 1), (n >> 1 & 1) ^ 1, 4u);
+    auto end_part = [&](int part) {
+      const Key key = run.best > -INFINITY ? argmax_key(run.best + 0.0f, run.at) : 0;
+      left.best[part][tid] = key;
+      most = key > most ? key : most;
+      run.best = -INFINITY;
+    };
+    const int loose = w.loose(tid), part_turns = w.part_turns(), parts = max(1, (w.turns() + part_turns - 1) / part_turns);
     if (loose >= 0 && loose < w.head) {
       const float v[1][1] = {{to_f32(w.x[loose])}};
       run.add(v, loose, 0);
     }
-    for (int i = 0; i < n_tiles; ++i) {
-      const int first = w.tile(warp, i) * kTile;
-      const int pieces = min(kTile, w.chunks - first);
+    // (two loops: the inner one holds nothing but the tile's work)
+    int pieces = w.chunks - w.tile(warp, 0) * kTile;                       // of the row, from the warp's next tile on
+    int last = w.chunk_first(w.tile(warp, 0) * kTile + lane) + N - 1;  // index of the lane's first piece's last element
+    const int step = w.step() * kTile;
+#pragma unroll 1
+    for (int part = 0; part < parts; ++part) {
+#pragma unroll 1
+    for (int i = 0; i < part_turns && pieces > 0; ++i) {
       wait(bars + stage, phase, 1u);
       Chunk<T> y[kUnroll];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) y[u].load_shared(ring + stage * kTileBytes + (u * 32 + lane) * 16);
       __syncwarp();
       if (fill_row < a.rows) fill(stage);
-      if (pieces == kTile) {
-        float v[kUnroll][N];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) y[u].get(v[u]);
-        run.add(v, w.chunk_first(first + lane) + N - 1, 32 * N);
-      } else {
+      if (pieces < kTile) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
-          if (u * 32 + lane < pieces) {
-            float v[1][N];
-            y[u].get(v[0]);
-            run.add(v, w.chunk_first(first + u * 32 + lane) + N - 1, 0);
-          }
+          if (u * 32 + lane >= pieces) y[u].clear();
       }
+      float v[kUnroll][N];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) y[u].get(v[u]);
+      run.add(v, last, 32 * N);
+      pieces -= step;
+      last += step * N;
       if (++stage == kStages) {
         stage = 0;
         phase ^= 1;
       }
     }
-    if (loose >= w.head) {
+    if (part + 1 == parts && loose >= w.head) {
       const float v[1][1] = {{to_f32(w.x[loose])}};
       run.add(v, loose, 0);
     }
+    if (a.top_k) end_part(part);
+    }
 
     if constexpr (!CLUSTER) {
-      wait(sh.empty + (n & 1), (n >> 1 & 1) ^ 1, 4u);
-      leave(run, a.top_k, sh.row[n & 1]);
+      leave(w, run, most, a.top_k, left);
       __syncwarp();
       if (lane == 0) mbar_arrive(sh.full + (n & 1));
     } else {
       const float given = token >= 0 && token < a.vocab ? to_f32(w.x[token]) : 0.0f;
-      leave(run, a.top_k, sh.row[0]);
+      leave(w, run, most, a.top_k, left);
       __syncthreads();
       // (every warp joins the warps' sums; lanes beyond them bring nothing)
       Sums sum = warp_join(lane < kWarps ? sh.row[0].sums[lane] : Sums{-FLT_MAX, 0.0f, 0.0f});
@@ -634,11 +663,12 @@ tl_status logprob_launch(const LogprobArgs& a, cudaStream_t s) {
       return TL_ERR_CUDA;
     ready[dev] = true;
   }
-  // A row is split over a cluster while that leaves no SM more than three CTAs
-  // and every thread at least two pieces.
+  // A row is split over a cluster while there are fewer CTAs than two an SM
+  // and every warp has a tile.
   int ctas = 1;
-  const int64_t rounds = (static_cast<int64_t>(a.vocab) * sizeof(T) / 16 + kThreads - 1) / kThreads;
-  while (ctas < kMaxCluster && static_cast<int64_t>(a.rows) * ctas * 2 <= device_sm_count() * 3 && rounds > ctas * 2)
+  const int64_t tiles = static_cast<int64_t>(a.vocab) * sizeof(T) / kTileBytes;
+  while (ctas < kMaxCluster && static_cast<int64_t>(a.rows) * ctas <= device_sm_count() &&
+         tiles + kWarps / 2 >= ctas * 2 * kWarps)
     ctas *= 2;
   if (ctas == 1) {
     const int grid = std::min(a.rows, device_sm_count() * kRowCtas);

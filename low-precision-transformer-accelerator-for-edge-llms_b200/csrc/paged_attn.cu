@@ -627,7 +627,9 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
       vinv = 0.0f;
     }
 
-    if (late ? !mbar_try_wait(bars + stage, phase) : !mbar_wait_err(bars + stage, phase, 1u, &g_paged_error)) late = true;
+    // (the clock is read only if there is something to wait for)
+    if (!mbar_try_wait(bars + stage, phase) && (late || !mbar_wait_err(bars + stage, phase, 1u, &g_paged_error)))
+      late = true;
     if constexpr (S::I8) cp_async_wait<S::STAGES - 1>();
     __syncwarp();
     const uint32_t kbase = ring32 + stage * S::STAGE, vbase = kbase + S::HALF;
