@@ -573,46 +573,47 @@ __global__ void __launch_bounds__(CLUSTER ? kThreads : kThreads + kPostWarps * 3
       most = key > most ? key : most;
       run.best = -INFINITY;
     };
-    const int loose = w.loose(tid), part_turns = w.part_turns(), parts = max(1, (w.turns() + part_turns - 1) / part_turns);
+    const int loose = w.loose(tid), part_turns = w.part_turns();
+    const int parts = max(1, (w.turns() + part_turns - 1) / part_turns);
     if (loose >= 0 && loose < w.head) {
       const float v[1][1] = {{to_f32(w.x[loose])}};
       run.add(v, loose, 0);
     }
     // (two loops: the inner one holds nothing but the tile's work)
-    int pieces = w.chunks - w.tile(warp, 0) * kTile;                       // of the row, from the warp's next tile on
-    int last = w.chunk_first(w.tile(warp, 0) * kTile + lane) + N - 1;  // index of the lane's first piece's last element
+    int pieces = w.chunks - w.tile(warp, 0) * kTile;  // of the row, from the warp's next tile on
+    int last = w.chunk_first(w.tile(warp, 0) * kTile + lane) + N - 1;  // last element of the lane's first piece
     const int step = w.step() * kTile;
 #pragma unroll 1
     for (int part = 0; part < parts; ++part) {
 #pragma unroll 1
-    for (int i = 0; i < part_turns && pieces > 0; ++i) {
-      wait(bars + stage, phase, 1u);
-      Chunk<T> y[kUnroll];
+      for (int i = 0; i < part_turns && pieces > 0; ++i) {
+        wait(bars + stage, phase, 1u);
+        Chunk<T> y[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) y[u].load_shared(ring + stage * kTileBytes + (u * 32 + lane) * 16);
-      __syncwarp();
-      if (fill_row < a.rows) fill(stage);
-      if (pieces < kTile) {
+        for (int u = 0; u < kUnroll; ++u) y[u].load_shared(ring + stage * kTileBytes + (u * 32 + lane) * 16);
+        __syncwarp();
+        if (fill_row < a.rows) fill(stage);
+        if (pieces < kTile) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-          if (u * 32 + lane >= pieces) y[u].clear();
+          for (int u = 0; u < kUnroll; ++u)
+            if (u * 32 + lane >= pieces) y[u].clear();
+        }
+        float v[kUnroll][N];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) y[u].get(v[u]);
+        run.add(v, last, 32 * N);
+        pieces -= step;
+        last += step * N;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
-      float v[kUnroll][N];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) y[u].get(v[u]);
-      run.add(v, last, 32 * N);
-      pieces -= step;
-      last += step * N;
-      if (++stage == kStages) {
-        stage = 0;
-        phase ^= 1;
+      if (part + 1 == parts && loose >= w.head) {
+        const float v[1][1] = {{to_f32(w.x[loose])}};
+        run.add(v, loose, 0);
       }
-    }
-    if (part + 1 == parts && loose >= w.head) {
-      const float v[1][1] = {{to_f32(w.x[loose])}};
-      run.add(v, loose, 0);
-    }
-    if (a.top_k) end_part(part);
+      if (a.top_k) end_part(part);
     }
 
     if constexpr (!CLUSTER) {

@@ -10,7 +10,8 @@
 // What bounds it. Each key and value byte is read once and used by the
 // group's query heads only (a few operations a byte), so the bound is the
 // rate of reading the pool. Everything else has to hide behind the loads:
-//  * work is split evenly over the CTAs whatever the lengths are (below);
+//  * work is split evenly over the CTAs whatever the lengths are (below, at
+//    attend_kernel);
 //  * each warp owns a ring of tiles that TMA fills ahead of it (boxes of rows
 //    of one page, 128-byte swizzle), so that no instruction of the warp moves
 //    data and ldmatrix reads the operands without bank conflicts;
@@ -29,7 +30,6 @@
 // per-row scales multiply the scores and the probabilities in float32.
 // Accumulators, maxima and sums are float32.
 #include <algorithm>
-
 #include <numeric>
 
 #include "kernels.cuh"
@@ -39,24 +39,6 @@
 namespace tl {
 namespace {
 
-#ifndef VAR_S64
-#define VAR_S64 3
-#endif
-#ifndef VAR_S128
-#define VAR_S128 2
-#endif
-#ifndef VAR_S256
-#define VAR_S256 2
-#endif
-#ifndef VAR_C64
-#define VAR_C64 3
-#endif
-#ifndef VAR_C128
-#define VAR_C128 2
-#endif
-#ifndef VAR_C256
-#define VAR_C256 2
-#endif
 constexpr int kWarps = 4;         // warps of a CTA, each on its own tiles
 constexpr int kMaxCtas = 640;     // grid bound (148 SMs x 4 CTAs), sizes the workspace
 constexpr float kLog2e = 1.4426950408889634f;
@@ -87,7 +69,8 @@ struct AttendArgs {
 };
 
 TL_DEV void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src))
+               : "memory");
 }
 TL_DEV void cp_async4(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)),
@@ -173,8 +156,15 @@ struct Shape {
   static constexpr int MERGE = HEADS * D * 4;           // a warp's partial result
   static constexpr int STAGE = 2 * HALF;
   static_assert(STAGE % 1024 == 0 && (KT * SUB) % 1024 == 0, "swizzled boxes");
-  static constexpr int STAGES = RB == 64 ? VAR_S64 : RB == 128 ? VAR_S128 : VAR_S256;
-  // shared memory: rings, the warps' partial results, the query's parts, then scales (int8), tile masks, partial m and l, query scales, barriers
+  // Tiles of a warp under way and CTAs an SM holds. One context of 131149
+  // positions (bf16, heads of 128): 2 tiles and 2 CTAs 96.5 us, 3 tiles and 2
+  // CTAs 151 (one CTA fits), 2 tiles and 3 CTAs 129 (168 registers spill); 64
+  // contexts up to 2048 over INT8 heads of 64: 2 tiles and 3 CTAs 20.5 us, 4
+  // tiles and 2 CTAs 23.8.
+  static constexpr int STAGES = 2;
+  static constexpr int CTAS = MT == 1 && RB == 64 ? 3 : 2;
+  // Shared memory: rings, the warps' partial results, the query's parts, then
+  // scales (int8), tile masks, partial m and l, query scales, barriers.
   static constexpr int RING = kWarps * STAGES * STAGE;
   static constexpr int QROW = D * 2;                    // bytes of a query row in 16 bits
   static constexpr int QTILE = 16 * QROW, QTHIRD = PARTS == 3 ? 8 * QROW : 0;
@@ -194,7 +184,6 @@ struct Shape {
   // 1, 2 and 3; 64 up to 2048 over INT8 22.9, 21.1, 21.8, 21.7.
   static constexpr int GAP = RB == 256 ? 3 : RB == 128 ? 2 : 1;
   static constexpr int RECORD = HEADS * (D + 2);        // floats of a partial result in the workspace
-  static constexpr int CTAS = MT == 2 ? 2 : RB == 64 ? VAR_C64 : RB == 128 ? VAR_C128 : VAR_C256;  // CTAs an SM holds
 };
 
 // Length of row r in positions, 0 for rows that name no sequence.
@@ -273,7 +262,7 @@ __device__ void join_records(const AttendArgs& a, unsigned char* smem, int4 x) {
   // weights in shared memory, and every thread sums its columns. It runs after
   // all other work of the item, so its few rounds of L2 latency show: as many
   // loads as registers allow are in flight, the first ones before the weights
-  // are known (37 records of 8 x 128: {T_JOIN}).
+  // are known (37 records of 8 x 128: about 4 us; 2 records 2 us).
   constexpr int COLS = S::HEADS * D / (kWarps * 128), BATCH = 64, DEPTH = (S::CTAS > 2 ? 16 : 32) / COLS;
   float* weight = reinterpret_cast<float*>(smem + S::PARTS_AT);  // [head][record]
   float* top = reinterpret_cast<float*>(smem + S::STATS);        // [head]: maximum, sum, factor of the old sums
@@ -609,221 +598,221 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
   // The first STAGES turns only fill the ring.
   for (int i = -S::STAGES, stage = 0, phase = 1; i < 0 || use.v < u1; ++i) {
     if (i >= 0) {
-    if (fresh) {
-      fresh = false;
-      store_query();
-      __syncthreads();  // the query is there, the last item's partial results have been read
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        qscale[mt] = reinterpret_cast<const float*>(smem + S::QSCALE)[mt * 8 + g];
-        m[mt] = -INFINITY;
-        l[mt] = 0.0f;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.0f;
-      }
-      vu = 0.0f;
-      vinv = 0.0f;
-    }
-
-    // (the clock is read only if there is something to wait for)
-    if (!mbar_try_wait(bars + stage, phase) && (late || !mbar_wait_err(bars + stage, phase, 1u, &g_paged_error)))
-      late = true;
-    if constexpr (S::I8) cp_async_wait<S::STAGES - 1>();
-    __syncwarp();
-    const uint32_t kbase = ring32 + stage * S::STAGE, vbase = kbase + S::HALF;
-    const float* sc = scales + stage * 2 * KT;
-    const unsigned live = masks[stage];
-    constexpr unsigned full = KT == 32 ? 0xffffffffu : 0xffffu;
-    if constexpr (!S::I8) {
-      // values of positions that do not exist must not meet a probability of zero as a NaN
-      if (live != 0 && live != full) {
-        for (int r = 0; r < KT; ++r)
-          if (!(live >> r & 1) && lane < S::RB / 16)
-            *reinterpret_cast<uint4*>(ring + stage * S::STAGE + S::HALF + (lane / (S::SUB / 16) * KT + r) * S::SUB +
-                                      lane % (S::SUB / 16) * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();  // before TMA writes there again
-        __syncwarp();
-      }
-    }
-    if (live) {
-      // ---- scores: s[mt][j] of positions 8 j + 2 t, + 1 for head g
-      float s[MT][KT / 8][2];
-      float c[KT / 8][MT][4];
-#pragma unroll
-      for (int j = 0; j < KT / 8; ++j)
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) c[j][mt][0] = c[j][mt][1] = c[j][mt][2] = c[j][mt][3] = 0.0f;
-      // 64 bytes of a key row at a time: lane l reads row l % 8, piece l / 8
-#pragma unroll
-      for (int q = 0; q < S::RB / 64; ++q) {
-        uint4 w[KT / 8];
-#pragma unroll
-        for (int j = 0; j < KT / 8; ++j)
-          w[j] = ldmatrix4<false>(kbase + (q * 64 / S::SUB * KT + 8 * j) * S::SUB + (q * 64 % S::SUB ^ k_lane));
-#pragma unroll
-        for (int k = 0; k < (S::I8 ? 4 : 2); ++k) {
-          const int ks = q * (S::I8 ? 4 : 2) + k;
-          uint32_t qa[MT][4], third[S::PARTS == 3 ? MT : 1][4];
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            const uint32_t at = mt * (S::QTILE + S::QTHIRD) + (((2 * ks) ^ q_piece) << 4);
-            const uint4 y = ldmatrix4<false>(q_row + at);
-            qa[mt][0] = y.x, qa[mt][1] = y.y, qa[mt][2] = y.z, qa[mt][3] = y.w;
-            if constexpr (S::PARTS == 3) {
-              // rows 0-7 only: matrices 1 and 3 repeat 0 and 2 and are not used
-              const uint4 z = ldmatrix4<false>(q32 + S::QTILE + l8 * S::QROW + at);
-              third[mt][0] = z.x, third[mt][1] = 0u, third[mt][2] = z.z, third[mt][3] = 0u;
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < KT / 8; ++j) {
-            const uint32_t ww[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
-            uint32_t b0, b1;
-            if constexpr (S::I8) {
-              const uint32_t u = ww[k] ^ 0x80808080u;
-              b0 = bytes_to_half2(u, 0x4140);
-              b1 = bytes_to_half2(u, 0x4342);
-            } else {
-              b0 = ww[2 * k];
-              b1 = ww[2 * k + 1];
-            }
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              mma16<S::BF>(c[j][mt], qa[mt], b0, b1);
-              if constexpr (S::PARTS == 3) mma16<S::BF>(c[j][mt], third[mt], b0, b1);
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < KT / 8; ++j) {
-        float2 kscale = make_float2(1.0f, 1.0f);
-        if constexpr (S::I8) {
-          kscale = *reinterpret_cast<const float2*>(sc + 8 * j + 2 * t);
-        }
+      if (fresh) {
+        fresh = false;
+        store_query();
+        __syncthreads();  // the query is there, the last item's partial results have been read
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          float x = (c[j][mt][0] + c[j][mt][2]) * qscale[mt], y = (c[j][mt][1] + c[j][mt][3]) * qscale[mt];
-          if constexpr (S::I8) {
-            x *= kscale.x;
-            y *= kscale.y;
-          }
-          s[mt][j][0] = x;
-          s[mt][j][1] = y;
-        }
-      }
-      if (live != full)
-#pragma unroll
-        for (int j = 0; j < KT / 8; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (!(live >> (8 * j + 2 * t + e) & 1))
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) s[mt][j][e] = -INFINITY;
-      // ---- running reference
-      float vs[KT / 8][2];
-      float vtop = 0.0f;
-      if constexpr (S::I8) {
-#pragma unroll
-        for (int j = 0; j < KT / 8; ++j) {
-          const float2 w = *reinterpret_cast<const float2*>(sc + KT + 8 * j + 2 * t);
-          vs[j][0] = w.x;
-          vs[j][1] = w.y;
-          vtop = fmaxf(vtop, fmaxf(fabsf(vs[j][0]), fabsf(vs[j][1])));
-        }
-        vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
-        vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 2));
-      }
-      float top[MT];
-      bool grow = S::I8 && vtop > vu;
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        top[mt] = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < KT / 8; ++j) top[mt] = fmaxf(top[mt], fmaxf(s[mt][j][0], s[mt][j][1]));
-        top[mt] = fmaxf(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 1));
-        top[mt] = fmaxf(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 2)) - kHeadroom;
-        grow |= top[mt] > m[mt] + kLazy;
-      }
-      if (__any_sync(0xffffffffu, grow)) {
-        float vcorr = 1.0f;
-        if constexpr (S::I8) {
-          if (vtop > vu) {  // the power of two at or above vtop (kept within float32's normal range)
-            const uint32_t e = min(max((__float_as_uint(vtop) + 0x7fffffu) >> 23, 2u), 252u);
-            const float nu = __uint_as_float(e << 23);
-            vcorr = vu * __uint_as_float((254u - e) << 23);
-            vu = nu;
-            vinv = __uint_as_float((254u - e) << 23);
-          }
-        }
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          float corr = vcorr;
-          if (top[mt] > m[mt]) {
-            const float f = exp2_approx(m[mt] - top[mt]);  // 0 from -infinity
-            l[mt] *= f;
-            corr *= f;
-            m[mt] = top[mt];
-          }
+          qscale[mt] = reinterpret_cast<const float*>(smem + S::QSCALE)[mt * 8 + g];
+          m[mt] = -INFINITY;
+          l[mt] = 0.0f;
 #pragma unroll
           for (int n = 0; n < D / 8; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[mt][n][e] *= corr;
+            for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.0f;
+        }
+        vu = 0.0f;
+        vinv = 0.0f;
+      }
+
+      // (the clock is read only if there is something to wait for)
+      if (!mbar_try_wait(bars + stage, phase) && (late || !mbar_wait_err(bars + stage, phase, 1u, &g_paged_error)))
+        late = true;
+      if constexpr (S::I8) cp_async_wait<S::STAGES - 1>();
+      __syncwarp();
+      const uint32_t kbase = ring32 + stage * S::STAGE, vbase = kbase + S::HALF;
+      const float* sc = scales + stage * 2 * KT;
+      const unsigned live = masks[stage];
+      constexpr unsigned full = KT == 32 ? 0xffffffffu : 0xffffu;
+      if constexpr (!S::I8) {
+        // values of positions that do not exist must not meet a probability of zero as a NaN
+        if (live != 0 && live != full) {
+          for (int r = 0; r < KT; ++r)
+            if (!(live >> r & 1) && lane < S::RB / 16)
+              *reinterpret_cast<uint4*>(ring + stage * S::STAGE + S::HALF + (lane / (S::SUB / 16) * KT + r) * S::SUB +
+                                        lane % (S::SUB / 16) * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();  // before TMA writes there again
+          __syncwarp();
         }
       }
-      // ---- probabilities, high and low rows
-      uint32_t pa[MT][KT / 16][4];
-      uint32_t pc[S::PARTS == 3 ? MT : 1][KT / 16][2];
+      if (live) {
+        // ---- scores: s[mt][j] of positions 8 j + 2 t, + 1 for head g
+        float s[MT][KT / 8][2];
+        float c[KT / 8][MT][4];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const float ref = m[mt] == -INFINITY ? 0.0f : m[mt];
+        for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) c[j][mt][0] = c[j][mt][1] = c[j][mt][2] = c[j][mt][3] = 0.0f;
+        // 64 bytes of a key row at a time: lane l reads row l % 8, piece l / 8
+#pragma unroll
+        for (int q = 0; q < S::RB / 64; ++q) {
+          uint4 w[KT / 8];
+#pragma unroll
+          for (int j = 0; j < KT / 8; ++j)
+            w[j] = ldmatrix4<false>(kbase + (q * 64 / S::SUB * KT + 8 * j) * S::SUB + (q * 64 % S::SUB ^ k_lane));
+#pragma unroll
+          for (int k = 0; k < (S::I8 ? 4 : 2); ++k) {
+            const int ks = q * (S::I8 ? 4 : 2) + k;
+            uint32_t qa[MT][4], third[S::PARTS == 3 ? MT : 1][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              const uint32_t at = mt * (S::QTILE + S::QTHIRD) + (((2 * ks) ^ q_piece) << 4);
+              const uint4 y = ldmatrix4<false>(q_row + at);
+              qa[mt][0] = y.x, qa[mt][1] = y.y, qa[mt][2] = y.z, qa[mt][3] = y.w;
+              if constexpr (S::PARTS == 3) {
+                // rows 0-7 only: matrices 1 and 3 repeat 0 and 2 and are not used
+                const uint4 z = ldmatrix4<false>(q32 + S::QTILE + l8 * S::QROW + at);
+                third[mt][0] = z.x, third[mt][1] = 0u, third[mt][2] = z.z, third[mt][3] = 0u;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < KT / 8; ++j) {
+              const uint32_t ww[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+              uint32_t b0, b1;
+              if constexpr (S::I8) {
+                const uint32_t u = ww[k] ^ 0x80808080u;
+                b0 = bytes_to_half2(u, 0x4140);
+                b1 = bytes_to_half2(u, 0x4342);
+              } else {
+                b0 = ww[2 * k];
+                b1 = ww[2 * k + 1];
+              }
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                mma16<S::BF>(c[j][mt], qa[mt], b0, b1);
+                if constexpr (S::PARTS == 3) mma16<S::BF>(c[j][mt], third[mt], b0, b1);
+              }
+            }
+          }
+        }
 #pragma unroll
         for (int j = 0; j < KT / 8; ++j) {
-          float x = exp2_approx(s[mt][j][0] - ref), y = exp2_approx(s[mt][j][1] - ref);
-          l[mt] += x + y;
+          float2 kscale = make_float2(1.0f, 1.0f);
           if constexpr (S::I8) {
-            x *= vs[j][0] * vinv;
-            y *= vs[j][1] * vinv;
+            kscale = *reinterpret_cast<const float2*>(sc + 8 * j + 2 * t);
           }
-          pa[mt][j >> 1][2 * (j & 1)] = split<S::BF>(x, y);
-          pa[mt][j >> 1][2 * (j & 1) + 1] = split<S::BF>(x, y);
-          if constexpr (S::PARTS == 3) pc[mt][j >> 1][j & 1] = split<S::BF>(x, y);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            float x = (c[j][mt][0] + c[j][mt][2]) * qscale[mt], y = (c[j][mt][1] + c[j][mt][3]) * qscale[mt];
+            if constexpr (S::I8) {
+              x *= kscale.x;
+              y *= kscale.y;
+            }
+            s[mt][j][0] = x;
+            s[mt][j][1] = y;
+          }
         }
-      }
-      // ---- o += p v
-      auto mma_pv = [&](int kk, int n, uint32_t b0, uint32_t b1) {
+        if (live != full)
+#pragma unroll
+          for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (!(live >> (8 * j + 2 * t + e) & 1))
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[mt][j][e] = -INFINITY;
+        // ---- running reference
+        float vs[KT / 8][2];
+        float vtop = 0.0f;
+        if constexpr (S::I8) {
+#pragma unroll
+          for (int j = 0; j < KT / 8; ++j) {
+            const float2 w = *reinterpret_cast<const float2*>(sc + KT + 8 * j + 2 * t);
+            vs[j][0] = w.x;
+            vs[j][1] = w.y;
+            vtop = fmaxf(vtop, fmaxf(fabsf(vs[j][0]), fabsf(vs[j][1])));
+          }
+          vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
+          vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 2));
+        }
+        float top[MT];
+        bool grow = S::I8 && vtop > vu;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          mma16<S::BF>(o[mt][n], pa[mt][kk], b0, b1);
-          if constexpr (S::PARTS == 3) {
-            const uint32_t third[4] = {pc[mt][kk][0], 0u, pc[mt][kk][1], 0u};
-            mma16<S::BF>(o[mt][n], third, b0, b1);
-          }
+          top[mt] = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < KT / 8; ++j) top[mt] = fmaxf(top[mt], fmaxf(s[mt][j][0], s[mt][j][1]));
+          top[mt] = fmaxf(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 1));
+          top[mt] = fmaxf(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 2)) - kHeadroom;
+          grow |= top[mt] > m[mt] + kLazy;
         }
-      };
-      // 32 bytes of 16 value rows at a time, transposed: lane l reads row l % 16, piece l / 16
-#pragma unroll
-      for (int kk = 0; kk < KT / 16; ++kk)
-#pragma unroll
-        for (int q = 0; q < S::RB / 32; ++q) {
-          const uint4 w = ldmatrix4<true>(vbase + (q * 32 / S::SUB * KT + 16 * kk) * S::SUB +
-                                          (q * 32 % S::SUB ^ v_lane));
+        if (__any_sync(0xffffffffu, grow)) {
+          float vcorr = 1.0f;
           if constexpr (S::I8) {
-            // a register holds elements 2 g, 2 g + 1 of position 2 t, then of 2 t + 1
-            const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              mma_pv(kk, 4 * q + 2 * h, bytes_to_half2(u[2 * h], 0x4240), bytes_to_half2(u[2 * h + 1], 0x4240));
-              mma_pv(kk, 4 * q + 2 * h + 1, bytes_to_half2(u[2 * h], 0x4341), bytes_to_half2(u[2 * h + 1], 0x4341));
+            if (vtop > vu) {  // the power of two at or above vtop (kept within float32's normal range)
+              const uint32_t e = min(max((__float_as_uint(vtop) + 0x7fffffu) >> 23, 2u), 252u);
+              const float nu = __uint_as_float(e << 23);
+              vcorr = vu * __uint_as_float((254u - e) << 23);
+              vu = nu;
+              vinv = __uint_as_float((254u - e) << 23);
             }
-          } else {
-            mma_pv(kk, 2 * q, w.x, w.y);
-            mma_pv(kk, 2 * q + 1, w.z, w.w);
+          }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            float corr = vcorr;
+            if (top[mt] > m[mt]) {
+              const float f = exp2_approx(m[mt] - top[mt]);  // 0 from -infinity
+              l[mt] *= f;
+              corr *= f;
+              m[mt] = top[mt];
+            }
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[mt][n][e] *= corr;
           }
         }
-    }
+        // ---- probabilities, high and low rows
+        uint32_t pa[MT][KT / 16][4];
+        uint32_t pc[S::PARTS == 3 ? MT : 1][KT / 16][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const float ref = m[mt] == -INFINITY ? 0.0f : m[mt];
+#pragma unroll
+          for (int j = 0; j < KT / 8; ++j) {
+            float x = exp2_approx(s[mt][j][0] - ref), y = exp2_approx(s[mt][j][1] - ref);
+            l[mt] += x + y;
+            if constexpr (S::I8) {
+              x *= vs[j][0] * vinv;
+              y *= vs[j][1] * vinv;
+            }
+            pa[mt][j >> 1][2 * (j & 1)] = split<S::BF>(x, y);
+            pa[mt][j >> 1][2 * (j & 1) + 1] = split<S::BF>(x, y);
+            if constexpr (S::PARTS == 3) pc[mt][j >> 1][j & 1] = split<S::BF>(x, y);
+          }
+        }
+        // ---- o += p v
+        auto mma_pv = [&](int kk, int n, uint32_t b0, uint32_t b1) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16<S::BF>(o[mt][n], pa[mt][kk], b0, b1);
+            if constexpr (S::PARTS == 3) {
+              const uint32_t third[4] = {pc[mt][kk][0], 0u, pc[mt][kk][1], 0u};
+              mma16<S::BF>(o[mt][n], third, b0, b1);
+            }
+          }
+        };
+        // 32 bytes of 16 value rows at a time, transposed: lane l reads row l % 16, piece l / 16
+#pragma unroll
+        for (int kk = 0; kk < KT / 16; ++kk)
+#pragma unroll
+          for (int q = 0; q < S::RB / 32; ++q) {
+            const uint4 w = ldmatrix4<true>(vbase + (q * 32 / S::SUB * KT + 16 * kk) * S::SUB +
+                                            (q * 32 % S::SUB ^ v_lane));
+            if constexpr (S::I8) {
+              // a register holds elements 2 g, 2 g + 1 of position 2 t, then of 2 t + 1
+              const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                mma_pv(kk, 4 * q + 2 * h, bytes_to_half2(u[2 * h], 0x4240), bytes_to_half2(u[2 * h + 1], 0x4240));
+                mma_pv(kk, 4 * q + 2 * h + 1, bytes_to_half2(u[2 * h], 0x4341), bytes_to_half2(u[2 * h + 1], 0x4341));
+              }
+            } else {
+              mma_pv(kk, 2 * q, w.x, w.y);
+              mma_pv(kk, 2 * q + 1, w.z, w.w);
+            }
+          }
+      }
 
     }
 
