@@ -117,6 +117,13 @@ TL_DEV void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// 16 x 8 += 16 x 32 of int8 and 32 x 8.
+TL_DEV void mma_s8(int* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 // (x, y) as two 16-bit values, and what the rounding left over in x, y.
 template <bool BF>
 TL_DEV uint32_t split(float& x, float& y) {
@@ -151,7 +158,7 @@ struct Shape {
   static constexpr int KT = RB == 256 ? 16 : 32;        // positions of a warp's tile
   static constexpr int SUB = RB < 128 ? RB : 128;       // bytes of a row in one box
   static constexpr int NSUB = RB / SUB;
-  static constexpr int KS = D / 16;                     // MMA steps over head_dim
+  static constexpr int KS = D / (I8 ? 32 : 16);         // steps of the first product over head_dim
   static constexpr int HALF = KT * RB;                  // bytes of a tile's keys, of its values
   static constexpr int MERGE = HEADS * D * 4;           // a warp's partial result
   static constexpr int STAGE = 2 * HALF;
@@ -166,8 +173,9 @@ struct Shape {
   // Shared memory: rings, the warps' partial results, the query's parts, then
   // scales (int8), tile masks, partial m and l, query scales, barriers.
   static constexpr int RING = kWarps * STAGES * STAGE;
-  static constexpr int QROW = D * 2;                    // bytes of a query row in 16 bits
-  static constexpr int QTILE = 16 * QROW, QTHIRD = PARTS == 3 ? 8 * QROW : 0;
+  static constexpr bool THIRD = I8 || PARTS == 3;       // the query has a third part
+  static constexpr int QROW = I8 ? D : D * 2;           // bytes of a part of a head's query
+  static constexpr int QTILE = 16 * QROW, QTHIRD = THIRD ? 8 * QROW : 0;
   static constexpr int PARTS_AT = RING;
   static constexpr int QUERY = PARTS_AT + kWarps * MERGE;  // [m tile]: 16 rows (8 high, 8 low), then 8 third rows
   static constexpr int SCALES = QUERY + MT * (QTILE + QTHIRD);
@@ -194,31 +202,32 @@ TL_DEV int row_length(const AttendArgs& a, int r, int* seq) {
   return s < 0 || s >= a.c.n_seqs ? 0 : max(0, min(n, a.c.max_pages * a.c.ps));
 }
 
-// A place on the line: round `rd` of item `it` (kv head and head block) of row
-// r, whose items have `units` rounds; v is its number on the line.
+// A place on the line: round `rd` of the item of kv head `kvh` and head block
+// `hb` of row r, whose items have `units` rounds; v is its number on the line.
 struct Place {
-  int r, seq, len, units, it, rd, v;
-  template <int UNIT>
-  TL_DEV void row(const AttendArgs& a, int row) {
+  int r, len, units, kvh, hb, rd, v;
+  const int32_t* pages;  // the row's block table
+
+  TL_DEV void row(const AttendArgs& a, int row, int seq, int length, int unit) {
     r = row;
-    len = 0;
-    units = 0;
-    while (r < a.rows) {
-      len = row_length(a, r, &seq);
-      units = (len + UNIT - 1) / UNIT;
-      if (units) break;
-      ++r;
-    }
+    len = length;
+    units = (length + unit - 1) / unit;
+    pages = a.c.table + static_cast<int64_t>(seq) * a.c.table_stride;
   }
   template <int UNIT, int GAP>
-  TL_DEV void next(const AttendArgs& a, int items) {
+  TL_DEV void next(const AttendArgs& a) {
     ++v;
     if (++rd < units) return;
     v += GAP;
     rd = 0;
-    if (++it < items) return;
-    it = 0;
-    row<UNIT>(a, r + 1);
+    if (++hb < a.blocks) return;
+    hb = 0;
+    if (++kvh < a.c.hkv) return;
+    kvh = 0;
+    int length = 0, seq = 0, row_ = r;
+    while (++row_ < a.rows && (length = row_length(a, row_, &seq)) == 0) {
+    }
+    row(a, row_, length ? seq : 0, length, UNIT);
   }
 };
 
@@ -429,18 +438,18 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
   }
   __syncthreads();
   Place use;
-  use.r = sh_first.x;
-  use.seq = sh_first.z;
-  use.len = sh_first.w;
-  use.units = (use.len + UNIT - 1) / UNIT;
-  use.it = (u0 - sh_first.y) / (use.units + S::GAP);
-  use.rd = (u0 - sh_first.y) - use.it * (use.units + S::GAP);
+  use.row(a, sh_first.x, sh_first.z, sh_first.w, UNIT);
+  {
+    const int item = (u0 - sh_first.y) / (use.units + S::GAP);
+    use.kvh = item / a.blocks;
+    use.hb = item - use.kvh * a.blocks;
+    use.rd = (u0 - sh_first.y) - item * (use.units + S::GAP);
+  }
   use.v = u0;
-  if (use.rd >= use.units) {  // in a gap
-    use.v += use.units + S::GAP - use.rd - 1;
-    use.v -= S::GAP;
+  if (use.rd >= use.units) {  // in a gap: on from the item's last round
+    use.v += use.units - 1 - use.rd;
     use.rd = use.units - 1;
-    use.next<UNIT, S::GAP>(a, items);
+    use.next<UNIT, S::GAP>(a);
   }
   if (use.v >= u1) {
     if (empty_row) zero_empty_rows<D>(a);
@@ -454,9 +463,9 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
   const int qh = tid / kLanes, qd = tid % kLanes * kQ;
   uint4 raw[kQ / 4];
   auto load_query = [&](const Place& p) {
-    const int kvh = p.it / a.blocks, hb = p.it - kvh * a.blocks;
-    const bool live = hb * S::HEADS + qh < a.group;
-    const int64_t base = p.r * a.ldq + static_cast<int64_t>(kvh * a.group + (live ? hb * S::HEADS + qh : 0)) * D + qd;
+    const bool live = p.hb * S::HEADS + qh < a.group;
+    const int64_t base =
+        p.r * a.ldq + static_cast<int64_t>(p.kvh * a.group + (live ? p.hb * S::HEADS + qh : 0)) * D + qd;
     const char* q = static_cast<const char*>(a.q) + base * (a.q_dtype == TL_F32 ? 4 : 2);
 #pragma unroll
     for (int e = 0; e < kQ / 4; ++e) raw[e] = make_uint4(0, 0, 0, 0);
@@ -483,32 +492,60 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
              : a.q_dtype == TL_BF16 ? __uint_as_float(half << 16)
                                     : __half2float(__ushort_as_half(static_cast<unsigned short>(half)));
     }
-    float f = 1.0f, back = a.scale * kLog2e;
+    // the scale's sign goes into the query, so that larger products are larger scores
+    float f = copysignf(1.0f, a.scale), back = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);
     if constexpr (!S::BF) {
-      // a power of two that takes the row's largest element to [2^10, 2^11)
+      // a power of two that takes the row's largest element to [2^10, 2^11), or [2^21, 2^22) for int8 digits
       float top = 0.0f;
+      bool bad = false;
 #pragma unroll
-      for (int e = 0; e < kQ; ++e) top = fmaxf(top, fabsf(x[e]));
+      for (int e = 0; e < kQ; ++e) {
+        top = fmaxf(top, fabsf(x[e]));
+        bad |= !(fabsf(x[e]) < INFINITY);
+      }
 #pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const int sh = max(-120, min(120, 10 - (static_cast<int>(__float_as_uint(top) >> 23) - 127)));
-      f = __int_as_float((127 + sh) << 23);
+      for (int o = 1; o < kLanes; o <<= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+      }
+      constexpr int kTop = S::I8 ? 21 : 10;
+      const int sh = max(-120, min(120, kTop - (static_cast<int>(__float_as_uint(top) >> 23) - 127)));
+      f *= __int_as_float((127 + sh) << 23);
       back *= __int_as_float((127 - sh) << 23);
+      if (bad) back = __int_as_float(0x7fc00000);  // a NaN or an infinity in the query makes the row NaN
     }
     if (qd == 0) reinterpret_cast<float*>(smem + S::QSCALE)[qh] = back;
     unsigned char* tile = smem + S::QUERY + (qh >> 3) * (S::QTILE + S::QTHIRD);
     const int row = qh & 7;
+    if constexpr (S::I8) {
+      // three signed digits to the base 256 of the element as a 22-bit integer
 #pragma unroll
-    for (int e = 0; e < kQ; e += 2) {
-      // column of the pair (d, d + 1): int8 keys bring elements 4 t .. 4 t + 3 to one lane
-      const int d = qd + e, j = d & 15;
-      const int col = S::I8 ? (d & ~15) + (j & 2) * 4 + (j >> 2) * 2 : d;
-      const int at = (((col >> 3) ^ row) << 4) + (col & 7) * 2;  // 16-byte pieces turned by the row
-      float u = x[e] * f, v = x[e + 1] * f;
-      *reinterpret_cast<uint32_t*>(tile + row * S::QROW + at) = split<S::BF>(u, v);
-      *reinterpret_cast<uint32_t*>(tile + (row + 8) * S::QROW + at) = split<S::BF>(u, v);
-      if constexpr (S::PARTS == 3)
-        *reinterpret_cast<uint32_t*>(tile + S::QTILE + row * S::QROW + at) = split<S::BF>(u, v);
+      for (int e = 0; e < kQ; e += 4) {
+        uint32_t d0 = 0, d1 = 0, d2 = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int v = __float2int_rn(x[e + i] * f);
+          const int v1 = (v - static_cast<int8_t>(v)) >> 8, v2 = (v1 - static_cast<int8_t>(v1)) >> 8;
+          d0 |= (v & 255) << (8 * i);
+          d1 |= (v1 & 255) << (8 * i);
+          d2 |= (v2 & 255) << (8 * i);
+        }
+        const int d = qd + e, turn = S::QROW == 128 ? row : row >> 1;  // (rows 8-15 turn as 0-7)
+        const int at = (((d >> 4) ^ turn) << 4) + (d & 15);
+        *reinterpret_cast<uint32_t*>(tile + row * S::QROW + at) = d2;
+        *reinterpret_cast<uint32_t*>(tile + (row + 8) * S::QROW + at) = d1;
+        *reinterpret_cast<uint32_t*>(tile + S::QTILE + row * S::QROW + at) = d0;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kQ; e += 2) {
+        const int d = qd + e, at = (((d >> 3) ^ row) << 4) + (d & 7) * 2;  // 16-byte pieces turned by the row
+        float u = x[e] * f, v = x[e + 1] * f;
+        *reinterpret_cast<uint32_t*>(tile + row * S::QROW + at) = split<S::BF>(u, v);
+        *reinterpret_cast<uint32_t*>(tile + (row + 8) * S::QROW + at) = split<S::BF>(u, v);
+        if constexpr (S::PARTS == 3)
+          *reinterpret_cast<uint32_t*>(tile + S::QTILE + row * S::QROW + at) = split<S::BF>(u, v);
+      }
     }
   };
   load_query(use);
@@ -528,11 +565,11 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
   // Row index of position `lane` of the tile at `p` (lanes < KT), -1: none.
   auto lookup = [&](const Place& p) -> int {
     const int pos = (p.rd * kWarps + warp) * KT + lane;
-    if (lane >= KT || p.units == 0 || pos >= p.len) return -1;
+    if (lane >= KT || pos >= p.len) return -1;
     const uint32_t pg = div_page(pos, a.c.div);
-    const int page = __ldg(a.c.table + static_cast<int64_t>(p.seq) * a.c.table_stride + pg);
-    if (page < 0 || page >= a.c.pages) return -1;
-    return (page * a.c.hkv + p.it / a.blocks) * a.c.ps + (pos - static_cast<int>(pg * a.c.div.d));
+    const int page = __ldg(p.pages + pg);
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.c.pages)) return -1;
+    return (page * a.c.hkv + p.kvh) * a.c.ps + (pos - static_cast<int>(pg * a.c.div.d));
   };
   // Boxes start at multiples of a.box positions and lie within one page, so a
   // box exists if its first position does (rows past the length stay unused).
@@ -582,7 +619,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
   const int l8 = lane & 7, v_row = lane & 15;
   const uint32_t q32 = smem_u32(smem + S::QUERY);
   // matrices of a query ldmatrix: rows 0-7, 8-15 of piece 2 k, then of piece 2 k + 1
-  const uint32_t q_row = q32 + v_row * S::QROW, q_piece = (lane >> 4) ^ l8;
+  const uint32_t q_row = q32 + v_row * S::QROW, q_piece = (lane >> 4) ^ (S::QROW == 64 ? l8 >> 1 : l8);
   const uint32_t k_lane = l8 * S::SUB + (((lane >> 3) ^ (S::SUB == 128 ? l8 : l8 >> 1)) << 4);
   const uint32_t v_lane = v_row * S::SUB + (((lane >> 4) ^ (S::SUB == 128 ? l8 : l8 >> 1)) << 4);
 
@@ -637,71 +674,90 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
         }
       }
       if (live) {
-        // ---- scores: s[mt][j] of positions 8 j + 2 t, + 1 for head g
+        // ---- products s[mt][j] of positions 8 j + 2 t, + 1 and head g, qscale times which are the scores
         float s[MT][KT / 8][2];
-        float c[KT / 8][MT][4];
-#pragma unroll
-        for (int j = 0; j < KT / 8; ++j)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) c[j][mt][0] = c[j][mt][1] = c[j][mt][2] = c[j][mt][3] = 0.0f;
+        uint32_t qa[MT][S::KS][4], third[S::THIRD ? MT : 1][S::KS][2];
+        auto load_q = [&](int mt, int ks) {
+          const uint32_t at = mt * (S::QTILE + S::QTHIRD) + (((2 * ks) ^ q_piece) << 4);
+          const uint4 y = ldmatrix4<false>(q_row + at);
+          qa[mt][ks][0] = y.x, qa[mt][ks][1] = y.y, qa[mt][ks][2] = y.z, qa[mt][ks][3] = y.w;
+          if constexpr (S::THIRD) {
+            // rows 0-7 only: matrices 1 and 3 repeat 0 and 2 and are not used
+            const uint4 z = ldmatrix4<false>(q32 + S::QTILE + l8 * S::QROW + at);
+            third[mt][ks][0] = z.x, third[mt][ks][1] = z.z;
+          }
+        };
         // 64 bytes of a key row at a time: lane l reads row l % 8, piece l / 8
+        auto load_k = [&](int j, int q) {
+          return ldmatrix4<false>(kbase + (q * 64 / S::SUB * KT + 8 * j) * S::SUB + (q * 64 % S::SUB ^ k_lane));
+        };
+        if constexpr (S::I8) {
 #pragma unroll
-        for (int q = 0; q < S::RB / 64; ++q) {
-          uint4 w[KT / 8];
+          for (int ks = 0; ks < S::KS; ++ks)
 #pragma unroll
-          for (int j = 0; j < KT / 8; ++j)
-            w[j] = ldmatrix4<false>(kbase + (q * 64 / S::SUB * KT + 8 * j) * S::SUB + (q * 64 % S::SUB ^ k_lane));
+            for (int mt = 0; mt < MT; ++mt) load_q(mt, ks);
 #pragma unroll
-          for (int k = 0; k < (S::I8 ? 4 : 2); ++k) {
-            const int ks = q * (S::I8 ? 4 : 2) + k;
-            uint32_t qa[MT][4], third[S::PARTS == 3 ? MT : 1][4];
+          for (int j = 0; j < KT / 8; ++j) {
+            int hi[MT][4], lo[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) hi[mt][e] = lo[mt][e] = 0;
+#pragma unroll
+            for (int q = 0; q < S::RB / 64; ++q) {
+              const uint4 w = load_k(j, q);
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                  const uint32_t low[4] = {third[mt][2 * q + k][0], 0u, third[mt][2 * q + k][1], 0u};
+                  mma_s8(hi[mt], qa[mt][2 * q + k], k ? w.z : w.x, k ? w.w : w.y);
+                  mma_s8(lo[mt], low, k ? w.z : w.x, k ? w.w : w.y);
+                }
+            }
+            const float2 kscale = *reinterpret_cast<const float2*>(sc + 8 * j + 2 * t);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              const uint32_t at = mt * (S::QTILE + S::QTHIRD) + (((2 * ks) ^ q_piece) << 4);
-              const uint4 y = ldmatrix4<false>(q_row + at);
-              qa[mt][0] = y.x, qa[mt][1] = y.y, qa[mt][2] = y.z, qa[mt][3] = y.w;
-              if constexpr (S::PARTS == 3) {
-                // rows 0-7 only: matrices 1 and 3 repeat 0 and 2 and are not used
-                const uint4 z = ldmatrix4<false>(q32 + S::QTILE + l8 * S::QROW + at);
-                third[mt][0] = z.x, third[mt][1] = 0u, third[mt][2] = z.z, third[mt][3] = 0u;
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < KT / 8; ++j) {
-              const uint32_t ww[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
-              uint32_t b0, b1;
-              if constexpr (S::I8) {
-                const uint32_t u = ww[k] ^ 0x80808080u;
-                b0 = bytes_to_half2(u, 0x4140);
-                b1 = bytes_to_half2(u, 0x4342);
-              } else {
-                b0 = ww[2 * k];
-                b1 = ww[2 * k + 1];
-              }
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                mma16<S::BF>(c[j][mt], qa[mt], b0, b1);
-                if constexpr (S::PARTS == 3) mma16<S::BF>(c[j][mt], third[mt], b0, b1);
-              }
+              // |sums| <= 128 * 128 * 127: the lower two digits' sum fits 31 bits, the whole is rounded once
+              s[mt][j][0] = fmaf(static_cast<float>(hi[mt][0]), 65536.0f, static_cast<float>(hi[mt][2] * 256 + lo[mt][0])) * kscale.x;
+              s[mt][j][1] = fmaf(static_cast<float>(hi[mt][1]), 65536.0f, static_cast<float>(hi[mt][3] * 256 + lo[mt][1])) * kscale.y;
             }
           }
-        }
+        } else {
+          float c[KT / 8][MT][4];
 #pragma unroll
-        for (int j = 0; j < KT / 8; ++j) {
-          float2 kscale = make_float2(1.0f, 1.0f);
-          if constexpr (S::I8) {
-            kscale = *reinterpret_cast<const float2*>(sc + 8 * j + 2 * t);
-          }
+          for (int j = 0; j < KT / 8; ++j)
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            float x = (c[j][mt][0] + c[j][mt][2]) * qscale[mt], y = (c[j][mt][1] + c[j][mt][3]) * qscale[mt];
-            if constexpr (S::I8) {
-              x *= kscale.x;
-              y *= kscale.y;
+            for (int mt = 0; mt < MT; ++mt) c[j][mt][0] = c[j][mt][1] = c[j][mt][2] = c[j][mt][3] = 0.0f;
+#pragma unroll
+          for (int q = 0; q < S::RB / 64; ++q) {
+            uint4 w[KT / 8];
+#pragma unroll
+            for (int j = 0; j < KT / 8; ++j) w[j] = load_k(j, q);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) load_q(mt, 2 * q + k);
+#pragma unroll
+              for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                  const uint32_t b0 = k ? w[j].z : w[j].x, b1 = k ? w[j].w : w[j].y;
+                  mma16<S::BF>(c[j][mt], qa[mt][2 * q + k], b0, b1);
+                  if constexpr (S::PARTS == 3) {
+                    const uint32_t low[4] = {third[mt][2 * q + k][0], 0u, third[mt][2 * q + k][1], 0u};
+                    mma16<S::BF>(c[j][mt], low, b0, b1);
+                  }
+                }
             }
-            s[mt][j][0] = x;
-            s[mt][j][1] = y;
           }
+#pragma unroll
+          for (int j = 0; j < KT / 8; ++j)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              s[mt][j][0] = c[j][mt][0] + c[j][mt][2];
+              s[mt][j][1] = c[j][mt][1] + c[j][mt][3];
+            }
         }
         if (live != full)
 #pragma unroll
@@ -733,7 +789,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
 #pragma unroll
           for (int j = 0; j < KT / 8; ++j) top[mt] = fmaxf(top[mt], fmaxf(s[mt][j][0], s[mt][j][1]));
           top[mt] = fmaxf(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 1));
-          top[mt] = fmaxf(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 2)) - kHeadroom;
+          top[mt] = fmaf(fmaxf(top[mt], __shfl_xor_sync(0xffffffffu, top[mt], 2)), qscale[mt], -kHeadroom);
           grow |= top[mt] > m[mt] + kLazy;
         }
         if (__any_sync(0xffffffffu, grow)) {
@@ -770,7 +826,8 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
           const float ref = m[mt] == -INFINITY ? 0.0f : m[mt];
 #pragma unroll
           for (int j = 0; j < KT / 8; ++j) {
-            float x = exp2_approx(s[mt][j][0] - ref), y = exp2_approx(s[mt][j][1] - ref);
+            float x = exp2_approx(fmaf(s[mt][j][0], qscale[mt], -ref));
+            float y = exp2_approx(fmaf(s[mt][j][1], qscale[mt], -ref));
             l[mt] += x + y;
             if constexpr (S::I8) {
               x *= vs[j][0] * vinv;
@@ -821,7 +878,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
     if (fill.v < u1) {
       copy_tile(stage, next_row);
       ++filled;
-      fill.next<UNIT, S::GAP>(a, items);
+      fill.next<UNIT, S::GAP>(a);
       next_row = fill.v < u1 ? lookup(fill) : -1;
     }
     if constexpr (S::I8) cp_async_commit();
@@ -860,15 +917,14 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
       }
       // the next item's query arrives while this one is joined
       const Place done = use;
-      use.next<UNIT, S::GAP>(a, items);
+      use.next<UNIT, S::GAP>(a);
       if (use.v < u1) load_query(use);
       __syncthreads();
-      const int kvh = done.it / a.blocks, hb = done.it - kvh * a.blocks;
-      const int nh = min(S::HEADS, a.group - hb * S::HEADS);
+      const int nh = min(S::HEADS, a.group - done.hb * S::HEADS);
       const int first = done.v - done.rd;  // the item's first round on the line
       const int c0 = first / chunk, c1 = (first + done.units - 1) / chunk;
       const bool whole = c0 == c1;
-      const int64_t head0 = static_cast<int64_t>(done.r) * a.heads + kvh * a.group + hb * S::HEADS;
+      const int64_t head0 = static_cast<int64_t>(done.r) * a.heads + done.kvh * a.group + done.hb * S::HEADS;
       float* rec = a.records + (static_cast<int64_t>(cta) * 2 + (cta == c0)) * S::RECORD;
 #pragma unroll 1
       for (int x = tid * 4; x < (whole ? nh : S::HEADS) * D; x += kWarps * 128) {
@@ -913,7 +969,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
       }
       fresh = true;
     } else if (i >= 0) {
-      use.next<UNIT, S::GAP>(a, items);
+      use.next<UNIT, S::GAP>(a);
     }
     if (++stage == S::STAGES) {
       stage = 0;
