@@ -267,17 +267,53 @@ __device__ void join_records(const AttendArgs& a, unsigned char* smem, int4 x) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int c0 = x.x, c1 = x.y, nh = x.w;
   const int64_t head0 = x.z;
+  constexpr int COLS = S::HEADS * D / (kWarps * 128), FEW = 6;
+  auto record = [&](int b) { return a.records + (static_cast<int64_t>(b) * 2 + (b == c0)) * S::RECORD; };
+  auto finish = [&](int c, float top, float sum, float4 v) {
+    const int h = (tid * 4 + c * kWarps * 128) / D, d = (tid * 4) % D;
+    if (h >= nh) return;
+    const bool empty = top == -INFINITY && sum == 0.0f;
+    const float inv = empty ? 0.0f : 1.0f / sum;
+    store_out(a.out, a.q_dtype, (head0 + h) * D + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    if (a.lse && d == 0) a.lse[head0 + h] = empty ? -INFINITY : (top + log2f(sum)) * kLn2;
+  };
+  if (c1 - c0 < FEW) {
+    // few records (a batch of ordinary contexts): every thread reads all that its column needs at once
+#pragma unroll 1
+    for (int c = 0; c < COLS; ++c) {
+      const int h = (tid * 4 + c * kWarps * 128) / D;
+      float bm[FEW], bl[FEW], top = -INFINITY, sum = 0.0f;
+      float4 y[FEW], v = make_float4(0, 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < FEW; ++k) {  // (past the end: the last one again)
+        const float* p = record(min(c0 + k, c1));
+        bm[k] = __ldcg(p + S::HEADS * D + h);
+        bl[k] = __ldcg(p + S::HEADS * D + S::HEADS + h);
+        y[k] = __ldcg(reinterpret_cast<const float4*>(p + tid * 4 + c * kWarps * 128));
+      }
+#pragma unroll
+      for (int k = 0; k < FEW; ++k) top = fmaxf(top, bm[k]);
+#pragma unroll
+      for (int k = 0; k < FEW; ++k)
+        if (c0 + k <= c1) {
+          const float e = bm[k] == -INFINITY ? 0.0f : exp2_approx(bm[k] - top);
+          sum += bl[k] * e;
+          v.x += y[k].x * e, v.y += y[k].y * e, v.z += y[k].z * e, v.w += y[k].w * e;
+        }
+      finish(c, top, sum, v);
+    }
+    return;
+  }
   // Of each batch of records, a warp a head turns the maxima and sums into
   // weights in shared memory, and every thread sums its columns. It runs after
   // all other work of the item, so its few rounds of L2 latency show: as many
   // loads as registers allow are in flight, the first ones before the weights
   // are known (37 records of 8 x 128: about 4 us; 2 records 2 us).
-  constexpr int COLS = S::HEADS * D / (kWarps * 128), BATCH = 64, DEPTH = (S::CTAS > 2 ? 16 : 32) / COLS;
+  constexpr int BATCH = 64, DEPTH = (S::CTAS > 2 ? 16 : 32) / COLS;
   float* weight = reinterpret_cast<float*>(smem + S::PARTS_AT);  // [head][record]
   float* top = reinterpret_cast<float*>(smem + S::STATS);        // [head]: maximum, sum, factor of the old sums
   float* sum = top + S::HEADS;
   float* old = sum + S::HEADS;
-  auto record = [&](int b) { return a.records + (static_cast<int64_t>(b) * 2 + (b == c0)) * S::RECORD; };
   float4 v[COLS], y[DEPTH][COLS];
   auto load = [&](int b, int end) {
 #pragma unroll
@@ -356,15 +392,14 @@ __device__ void join_records(const AttendArgs& a, unsigned char* smem, int4 x) {
     }
     __syncthreads();  // the weights have been used
   }
-#pragma unroll
+#pragma unroll 1
   for (int c = 0; c < COLS; ++c) {
-    const int h = (tid * 4 + c * kWarps * 128) / D, d = (tid * 4) % D;
-    if (h >= nh) continue;
-    const bool empty = top[h] == -INFINITY && sum[h] == 0.0f;
-    const float inv = empty ? 0.0f : 1.0f / sum[h];
-    store_out(a.out, a.q_dtype, (head0 + h) * D + d,
-              make_float4(v[c].x * inv, v[c].y * inv, v[c].z * inv, v[c].w * inv));
-    if (a.lse && d == 0) a.lse[head0 + h] = empty ? -INFINITY : (top[h] + log2f(sum[h])) * kLn2;
+    const int h = (tid * 4 + c * kWarps * 128) / D;
+    float4 x = v[0];
+#pragma unroll
+    for (int k = 1; k < COLS; ++k)
+      if (c == k) x = v[k];
+    finish(c, top[h], sum[h], x);
   }
 }
 
@@ -638,6 +673,12 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
       if (fresh) {
         fresh = false;
         store_query();
+        // the next item's query is on its way while this one's rounds run
+        Place ahead = use;
+        ahead.v += ahead.units - 1 - ahead.rd;
+        ahead.rd = ahead.units - 1;
+        if (ahead.v < u1) ahead.next<UNIT, S::GAP>(a);
+        if (ahead.v < u1) load_query(ahead);
         __syncthreads();  // the query is there, the last item's partial results have been read
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -915,10 +956,8 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
           }
         }
       }
-      // the next item's query arrives while this one is joined
       const Place done = use;
       use.next<UNIT, S::GAP>(a);
-      if (use.v < u1) load_query(use);
       __syncthreads();
       const int nh = min(S::HEADS, a.group - done.hb * S::HEADS);
       const int first = done.v - done.rd;  // the item's first round on the line
@@ -979,16 +1018,16 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
   if (pending) {
     // tickets are drawn at the end, when all parts are written: the CTA that
     // draws an item's last one joins its parts
-    __threadfence();
     __syncthreads();
     if (tid < pending) {
       const int4 x = tid ? late1 : late0;
+      __threadfence();  // the CTA's writes, ordered before by the barrier, before the ticket
       const bool last = atomicAdd(a.tickets + x.x, 1u) == static_cast<unsigned>(x.y - x.x);
       if (last) a.tickets[x.x] = 0;
+      __threadfence();  // the other CTAs' writes after it
       sh_last[tid] = last;
     }
     __syncthreads();
-    __threadfence();
 #pragma unroll 1
     for (int j = 0; j < pending; ++j)
       if (sh_last[j]) join_records<S>(a, smem, j ? late1 : late0);
