@@ -389,8 +389,9 @@ TL_API void* tl_engine_stream(tl_engine* eng);
  * (NULL = legacy default stream). Shapes must satisfy K % 16 == 0 and
  * 16-byte aligned int8 rows. */
 
-/* Waits for the device and reports TL_ERR_TIMEOUT if a tensor-core kernel
- * gave up on a bounded pipeline wait since the last call (then clears it). */
+/* Waits for the device and reports TL_ERR_TIMEOUT if a tensor-core kernel, the
+ * paged attention or the log probabilities gave up on a bounded wait for a copy
+ * since the last call (then clears it). Their results are void then. */
 TL_API tl_status tl_device_error(void);
 
 /* int8 W[K][N] -> W^T[N][K] (device to device). */
@@ -616,11 +617,12 @@ TL_API tl_status tl_paged_read(const tl_paged_kv* cache, const tl_paged_read_arg
  * positions whose page does not exist are left out; a row without positions
  * (length 0, padding) gives zeros and lse = -infinity. heads may be any
  * multiple of kv_heads. Sums and softmax statistics are float32; products run
- * on the tensor cores with the query and the probabilities split so that a
- * float32 query keeps float32 accuracy for every pool type.
- * workspace: tl_paged_attn_workspace_bytes bytes of device memory, 16-byte aligned, zeroed once
- * by the caller before its first call; every call leaves it ready for the
- * next. Calls that share one workspace must not overlap on the GPU. The call
+ * on the tensor cores with the query and the probabilities split into parts of
+ * fewer bits that add up to at least 22 of a float32 query's 24 bits (counted
+ * from its row's largest element) and 16 (TL_BF16) or 22 of a probability's.
+ * workspace: tl_paged_attn_workspace_bytes bytes of device memory, 16-byte
+ * aligned, zeroed once by the caller before its first call; every call leaves
+ * it ready for the next. Calls that share one workspace must not overlap on the GPU. The call
  * allocates nothing, does not synchronise and can be captured in a graph. */
 TL_API size_t tl_paged_attn_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t head_dim);
 typedef struct tl_paged_attn_args {

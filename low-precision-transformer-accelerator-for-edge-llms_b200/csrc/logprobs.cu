@@ -658,9 +658,9 @@ tl_status logprob_launch(const LogprobArgs& a, cudaStream_t s) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TL_ERR_CUDA;
   if (!ready[dev]) {
-    if (cudaFuncSetAttribute(logprob_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing) !=
-            cudaSuccess ||
-        cudaFuncSetAttribute(logprob_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing) != cudaSuccess)
+    const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    if (cudaFuncSetAttribute(logprob_kernel<T, false>, attr, kRing) != cudaSuccess ||
+        cudaFuncSetAttribute(logprob_kernel<T, true>, attr, kRing) != cudaSuccess)
       return TL_ERR_CUDA;
     ready[dev] = true;
   }

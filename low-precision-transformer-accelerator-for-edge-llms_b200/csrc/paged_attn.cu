@@ -15,20 +15,25 @@
 //  * each warp owns a ring of tiles that TMA fills ahead of it (boxes of rows
 //    of one page, 128-byte swizzle), so that no instruction of the warp moves
 //    data and ldmatrix reads the operands without bank conflicts;
-//  * both products run on mma.sync m16n8k16. A group has few rows, so a
-//    128-row tcgen05 tile would be mostly padding and its result would have
-//    to come back through tensor memory; the 16-row tile is small enough to
-//    stay far below the issue limit at full bandwidth.
+//  * both products run on mma.sync (m16n8k16, m16n8k32 for int8 keys). A group
+//    has few rows, so a 128-row tcgen05 tile would be mostly padding and its
+//    result would have to come back through tensor memory; the 16-row tile is
+//    small enough to stay below the issue limit at full bandwidth.
 //
-// Precision. A 16-row tile holds 8 query heads twice: row g is the high part
-// of head g's query (or of its probabilities), row g + 8 the low part, what
-// rounding the high part to 16 bits left over. The sum of the two rows of the
-// product is therefore the product with a 22-bit (float16) or 16-bit (bf16)
-// operand, for no more instructions than one part takes with <= 8 heads. For
-// a float32 query over a bf16 pool a third part (24 bits) takes a second MMA.
-// Keys and values are exact: int8 converts to float16 exactly and its
-// per-row scales multiply the scores and the probabilities in float32.
-// Accumulators, maxima and sums are float32.
+// Precision. Keys and values are exact, the other operand is split so that
+// nothing but its last bits is rounded; accumulators, maxima and sums are
+// float32.
+//  * A 16-row tile holds 8 heads twice: row g is the high part of head g's
+//    query (or of its probabilities), row g + 8 the low part, what rounding
+//    the high part to 16 bits left over. The sum of the two rows of the
+//    product is the product with a 22-bit (float16) or 16-bit (bf16) operand,
+//    for no more instructions than one part takes with <= 8 heads. For a
+//    float32 query over a bf16 pool a third part (24 bits) takes a second MMA.
+//  * Over an INT8 pool the query is a 22-bit integer times a power of two, as
+//    three signed digits to the base 256: two in the tile's rows, the third by
+//    a second MMA. Their sums are whole numbers. The probabilities are split as
+//    above and meet the values as float16, which holds every int8. The per-row
+//    scales multiply the scores and the probabilities in float32.
 #include <algorithm>
 #include <numeric>
 
@@ -65,7 +70,7 @@ struct AttendArgs {
   float* lse;
   int32_t box;            // rows of a TMA box: the largest that divides a page and a tile
   unsigned int* tickets;  // [kMaxCtas], zero between calls
-  float* records;         // [kMaxCtas][2][kHeads][D + 2]
+  float* records;         // [kMaxCtas][2]: a partial result (HEADS rows, maxima, sums)
 };
 
 TL_DEV void cp_async16(uint32_t dst, const void* src) {
@@ -163,11 +168,12 @@ struct Shape {
   static constexpr int MERGE = HEADS * D * 4;           // a warp's partial result
   static constexpr int STAGE = 2 * HALF;
   static_assert(STAGE % 1024 == 0 && (KT * SUB) % 1024 == 0, "swizzled boxes");
-  // Tiles of a warp under way and CTAs an SM holds. One context of 131149
-  // positions (bf16, heads of 128): 2 tiles and 2 CTAs 96.5 us, 3 tiles and 2
-  // CTAs 151 (one CTA fits), 2 tiles and 3 CTAs 129 (168 registers spill); 64
-  // contexts up to 2048 over INT8 heads of 64: 2 tiles and 3 CTAs 20.5 us, 4
-  // tiles and 2 CTAs 23.8.
+  // Tiles of a warp under way and CTAs an SM holds, each against the time of
+  // the kernel as it was then. One context of 131149 positions (bf16, heads of
+  // 128), 96.5 us: 3 tiles 151 (one CTA fits), 3 CTAs 129 (168 registers spill).
+  // 64 contexts up to 2048 over INT8 heads of 64, 20.4 us: 4 tiles and 2 CTAs
+  // 23.8, 4 CTAs 20.8 (256 contexts: 46.5, 49.5). Tiles of 16 positions take
+  // 62 us there.
   static constexpr int STAGES = 2;
   static constexpr int CTAS = MT == 1 && RB == 64 ? 3 : 2;
   // Shared memory: rings, the warps' partial results, the query's parts, then
@@ -187,9 +193,10 @@ struct Shape {
   static constexpr int UNIT = kWarps * KT;              // positions of one CTA round
   // What ending an item costs a CTA (its warps' results joined, the next query,
   // its part written), in rounds: the line leaves such a gap behind every item,
-  // so that CTAs that cross items get fewer rounds. 16 contexts up to 8192
-  // (float16, heads of 128) take 61.3 us with no gap, 54.6, 53.2 and 52.0 with
-  // 1, 2 and 3; 64 up to 2048 over INT8 22.9, 21.1, 21.8, 21.7.
+  // so that CTAs that cross items get fewer rounds. When the gaps came in, 16
+  // contexts up to 8192 (float16, heads of 128) took 61.3 us without them and
+  // 54.6, 53.2, 52.0 with 1, 2, 3; 64 up to 2048 over INT8 22.9 and 21.1, 21.8,
+  // 21.7.
   static constexpr int GAP = RB == 256 ? 3 : RB == 128 ? 2 : 1;
   static constexpr int RECORD = HEADS * (D + 2);        // floats of a partial result in the workspace
 };
@@ -261,6 +268,7 @@ TL_DEV void zero_empty_rows(const AttendArgs& a) {
 }
 
 // Joins the parts of an item, x = (first CTA, last CTA, first row of out, heads).
+// It runs after all other work of the item, so its rounds of L2 latency show.
 template <typename S>
 __device__ void join_records(const AttendArgs& a, unsigned char* smem, int4 x) {
   constexpr int D = S::D;
@@ -278,7 +286,8 @@ __device__ void join_records(const AttendArgs& a, unsigned char* smem, int4 x) {
     if (a.lse && d == 0) a.lse[head0 + h] = empty ? -INFINITY : (top + log2f(sum)) * kLn2;
   };
   if (c1 - c0 < FEW) {
-    // few records (a batch of ordinary contexts): every thread reads all that its column needs at once
+    // few records (a batch of ordinary contexts): every thread reads all that its column needs at once,
+    // one round of latency (64 contexts up to 2048 over INT8: 18.8 us, 20.4 by the way below)
 #pragma unroll 1
     for (int c = 0; c < COLS; ++c) {
       const int h = (tid * 4 + c * kWarps * 128) / D;
@@ -305,10 +314,9 @@ __device__ void join_records(const AttendArgs& a, unsigned char* smem, int4 x) {
     return;
   }
   // Of each batch of records, a warp a head turns the maxima and sums into
-  // weights in shared memory, and every thread sums its columns. It runs after
-  // all other work of the item, so its few rounds of L2 latency show: as many
-  // loads as registers allow are in flight, the first ones before the weights
-  // are known (37 records of 8 x 128: about 4 us; 2 records 2 us).
+  // weights in shared memory, and every thread sums its columns: as many loads
+  // as registers allow are in flight, the first ones before the weights are
+  // known (37 records of 8 x 128: about 4 us).
   constexpr int BATCH = 64, DEPTH = (S::CTAS > 2 ? 16 : 32) / COLS;
   float* weight = reinterpret_cast<float*>(smem + S::PARTS_AT);  // [head][record]
   float* top = reinterpret_cast<float*>(smem + S::STATS);        // [head]: maximum, sum, factor of the old sums
@@ -759,9 +767,13 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
             const float2 kscale = *reinterpret_cast<const float2*>(sc + 8 * j + 2 * t);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              // |sums| <= 128 * 128 * 127: the lower two digits' sum fits 31 bits, the whole is rounded once
-              s[mt][j][0] = fmaf(static_cast<float>(hi[mt][0]), 65536.0f, static_cast<float>(hi[mt][2] * 256 + lo[mt][0])) * kscale.x;
-              s[mt][j][1] = fmaf(static_cast<float>(hi[mt][1]), 65536.0f, static_cast<float>(hi[mt][3] * 256 + lo[mt][1])) * kscale.y;
+              // digits' sums are at most 128 * 128 * 127: the lower two together fit 31 bits; float32 rounds
+              // those and the whole once each
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float low = static_cast<float>(hi[mt][2 + e] * 256 + lo[mt][e]);
+                s[mt][j][e] = fmaf(static_cast<float>(hi[mt][e]), 65536.0f, low) * (e ? kscale.y : kscale.x);
+              }
             }
           }
         } else {
@@ -911,7 +923,6 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
             }
           }
       }
-
     }
 
     // ---- the tile has been read by all lanes: the next one for its place
@@ -1066,15 +1077,22 @@ tl_status attend_launch(AttendArgs& a, cudaStream_t s) {
 }
 
 // Groups of up to 8 query heads fit one 16-row tile, larger ones take two at a
-// time so that the pool is read once for every 16 heads.
+// time so that the pool is read once for every 16 heads: groups of 16 over one
+// context of 131149 positions (bf16, heads of 128) 74 us, 89 with one tile; 64
+// contexts up to 8192 over INT8 heads of 64, 63 and 72. INT8 heads of 128 take
+// one tile at a time: two spill registers, 53 us against 43 (64 contexts up to
+// 2048), 152 against 132 (256 of them).
 template <int POOL, int D, int PARTS>
 tl_status attend_heads(AttendArgs& a, cudaStream_t s) {
-  if (a.group <= 8) {
-    a.blocks = 1;
-    return attend_launch<Shape<POOL, D, 1, PARTS>>(a, s);
+  constexpr bool kTwo = !(POOL == TL_I8 && D == 128);
+  if constexpr (kTwo) {
+    if (a.group > 8) {
+      a.blocks = (a.group + 15) / 16;
+      return attend_launch<Shape<POOL, D, 2, PARTS>>(a, s);
+    }
   }
-  a.blocks = (a.group + 15) / 16;
-  return attend_launch<Shape<POOL, D, 2, PARTS>>(a, s);
+  a.blocks = (a.group + 7) / 8;
+  return attend_launch<Shape<POOL, D, 1, PARTS>>(a, s);
 }
 template <int POOL>
 tl_status attend_dim(AttendArgs& a, int d, cudaStream_t s) {
