@@ -39,13 +39,18 @@ _READ = Struct("@5Pq4i")
 _ATTEND = Struct("@7PN2q5if")
 _LOGPROBS = Struct("@6Pq4i")
 
-torch = None  # imported by the first call that needs it (importing the package does not)
+# Imported by the first call that needs it (importing the package does not).
+# Small calls are as long as their host side: what every call looks up is bound once.
+torch = _Tensor = _INT32 = _FLOAT32 = _device = _stream = None
 
 
 def _need_torch():
-    global torch
+    global torch, _Tensor, _INT32, _FLOAT32, _device, _stream
     if torch is None:
         import torch as module
+        _Tensor, _INT32, _FLOAT32 = module.Tensor, module.int32, module.float32
+        _device = module.cuda.current_device
+        _stream = getattr(module._C, "_cuda_getCurrentRawStream", None)  # (None without CUDA)
         torch = module
         _FLOAT_CODES.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
         _POOL_CODES.update({torch.int8: I8, torch.bfloat16: BF16, torch.float16: F16})
@@ -59,7 +64,7 @@ def _bad(name, t, want):
 
 def _index(name, t, n, gpu):
     """int32 vector of n entries on device ``gpu`` -> its address."""
-    if (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == (n,) and t.get_device() == gpu
+    if (isinstance(t, _Tensor) and t.dtype is _INT32 and t.shape == (n,) and t.get_device() == gpu
             and t.is_contiguous()):
         return t.data_ptr()
     raise _bad(name, t, f"a contiguous int32 [{n}] tensor on cuda:{gpu}")
@@ -67,7 +72,7 @@ def _index(name, t, n, gpu):
 
 def _rows(name, t, n, heads, d, dtype, gpu):
     """[n, heads, d] activations with contiguous head rows, 16-byte aligned -> (address, row stride)."""
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == (n, heads, d) and t.get_device() == gpu:
+    if isinstance(t, _Tensor) and t.dtype is dtype and t.shape == (n, heads, d) and t.get_device() == gpu:
         s0, s1, s2 = t.stride()
         p = t.data_ptr()
         if n < 2:
@@ -79,7 +84,7 @@ def _rows(name, t, n, heads, d, dtype, gpu):
 
 
 def _angles(name, t, rows, d, gpu):
-    if (isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.shape == (rows, d) and rows
+    if (isinstance(t, _Tensor) and t.dtype is _FLOAT32 and t.shape == (rows, d) and rows
             and t.get_device() == gpu and t.is_contiguous()):
         p = t.data_ptr()
         if not p & 15:
@@ -101,11 +106,11 @@ def _out(name, t, like, shape, dtype):
 
 def _enqueue(what, fn, gpu, *args):
     """Calls a library entry on the current stream of device ``gpu``, with that device current."""
-    if torch.cuda.current_device() == gpu:
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
+    if _device() == gpu:
+        code = fn(*args, _stream(gpu))
     else:
         with torch.cuda.device(gpu):
-            code = fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
+            code = fn(*args, _stream(gpu))
     if code:
         check(code, what)
 
@@ -184,7 +189,7 @@ class PagedKVCache:
 
     # ---------------------------------------------------------------- calls
     def _table(self, t):
-        if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 2 and t.get_device() == self._gpu:
+        if isinstance(t, _Tensor) and t.dtype is _INT32 and t.dim() == 2 and t.get_device() == self._gpu:
             n, m = t.shape
             stride, one = t.stride()
             if n < 2:
