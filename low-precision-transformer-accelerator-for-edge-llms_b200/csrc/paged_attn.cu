@@ -718,7 +718,6 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
             if (!(live >> r & 1) && lane < S::RB / 16)
               *reinterpret_cast<uint4*>(ring + stage * S::STAGE + S::HALF + (lane / (S::SUB / 16) * KT + r) * S::SUB +
                                         lane % (S::SUB / 16) * 16) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async_smem();  // before TMA writes there again
           __syncwarp();
         }
       }
@@ -925,7 +924,9 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
       }
     }
 
-    // ---- the tile has been read by all lanes: the next one for its place
+    // ---- the tile has been read by all lanes (a fence, since copies belong to the async proxy): the next one
+    // for its place
+    fence_proxy_async_smem();
     __syncwarp();
     if (fill.v < u1) {
       copy_tile(stage, next_row);
