@@ -507,6 +507,7 @@ __global__ void __launch_bounds__(CLUSTER ? kThreads : kThreads + kPostWarps * 3
     __syncwarp();
   else
     __syncthreads();
+  pdl_begin();
 
   if (!CLUSTER && warp >= kWarps) {
     // ---- results, a row behind
@@ -677,21 +678,10 @@ tl_status logprob_launch(const LogprobArgs& a, cudaStream_t s) {
     ctas *= 2;
   if (ctas == 1) {
     const int grid = std::min(a.rows, device_sm_count() * kRowCtas);
-    logprob_kernel<T, false><<<grid, kThreads + kPostWarps * 32, kRing, s>>>(a, 1);
-    return cuda_status(cudaGetLastError());
+    return launch_serving(logprob_kernel<T, false>, grid, kThreads + kPostWarps * 32, kRing, 1, s, a, 1);
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.rows) * ctas);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = kRing;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, logprob_kernel<T, true>, a, ctas));
+  const unsigned grid = static_cast<unsigned>(a.rows) * ctas;
+  return launch_serving(logprob_kernel<T, true>, grid, kThreads, kRing, ctas, s, a, ctas);
 }
 
 }  // namespace

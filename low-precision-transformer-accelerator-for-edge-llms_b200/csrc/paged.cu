@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
   const int g = static_cast<int>(part - static_cast<unsigned>(t) * a.groups);
   const bool in = t < a.tokens;  // (the row maxima below are warp-wide)
   const int rows = a.heads + 2 * a.c.hkv;
+  pdl_begin();
 
   const int p = in ? a.pos[t] : -1, s = in ? a.seq[t] : -1;  // the longest chain of loads starts here
   Raw<TI, N> in_lo[kRows], in_hi[kRows];
@@ -235,6 +236,7 @@ __global__ void __launch_bounds__(kThreads)
   const unsigned part = static_cast<unsigned>(id / LANES);
   const int64_t t = part / static_cast<unsigned>(groups);
   const int g = static_cast<int>(part - static_cast<unsigned>(t) * groups);
+  pdl_begin();
   if (t >= tokens) return;
   const int64_t row0 = paged_row(c, seq[t], pos[t]);
   Raw<TC, N> x[kRows];
@@ -279,8 +281,7 @@ template <typename TI, typename TC, int D>
 tl_status append_launch(AppendArgs& a, cudaStream_t s) {
   unsigned grid;
   if (!grid_for(a.tokens, a.heads + 2 * a.c.hkv, D / 2 * sizeof(TI) / 16, &a.groups, &grid)) return TL_ERR_OUT_OF_RANGE;
-  append_kernel<TI, TC, D><<<grid, kThreads, 0, s>>>(a);
-  return cuda_status(cudaGetLastError());
+  return launch_serving(append_kernel<TI, TC, D>, grid, kThreads, 0, 1, s, a);
 }
 template <typename TI, typename TC>
 tl_status append_dim(AppendArgs& a, int d, cudaStream_t s) {
@@ -304,9 +305,8 @@ tl_status read_launch(const ReadArgs& a, cudaStream_t s) {
   unsigned grid;
   int groups;
   if (!grid_for(a.tokens, 2 * a.c.hkv, D * sizeof(TO) / 16, &groups, &grid)) return TL_ERR_OUT_OF_RANGE;
-  read_kernel<TC, TO, D><<<grid, kThreads, 0, s>>>(a.c, a.seq, a.pos, a.tokens, groups, static_cast<TO*>(a.k),
-                                                   static_cast<TO*>(a.v));
-  return cuda_status(cudaGetLastError());
+  return launch_serving(read_kernel<TC, TO, D>, grid, kThreads, 0, 1, s, a.c, a.seq, a.pos, a.tokens, groups,
+                        static_cast<TO*>(a.k), static_cast<TO*>(a.v));
 }
 template <typename TC, typename TO>
 tl_status read_dim(const ReadArgs& a, int d, cudaStream_t s) {

@@ -435,6 +435,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
     prefetch_tensormap(&tm_k);
     prefetch_tensormap(&tm_v);
   }
+  pdl_begin();
   // ---- the CTA's stretch [u0, u1) of the line
   const int ctas = static_cast<int>(gridDim.x), cta = static_cast<int>(blockIdx.x);
   const int per = (a.rows + kWarps * 32 - 1) / (kWarps * 32);
@@ -1073,8 +1074,7 @@ tl_status attend_launch(AttendArgs& a, cudaStream_t s) {
   if (tc_encode_rows_bytes(&tm_k, a.c.k, pool_rows, S::RB, a.box) != cudaSuccess ||
       tc_encode_rows_bytes(&tm_v, a.c.v, pool_rows, S::RB, a.box) != cudaSuccess)
     return TL_ERR_CUDA;
-  attend_kernel<S><<<static_cast<unsigned>(grid), kWarps * 32, S::SMEM, s>>>(a, tm_k, tm_v);
-  return cuda_status(cudaGetLastError());
+  return launch_serving(attend_kernel<S>, static_cast<unsigned>(grid), kWarps * 32, S::SMEM, 1, s, a, tm_k, tm_v);
 }
 
 // Groups of up to 8 query heads fit one 16-row tile, larger ones take two at a

