@@ -113,7 +113,7 @@ TL_DEV void store_n(T* p, const float* x) {
 // the reference's values), and quantize_int8 of the whole row, whose maximum
 // is taken over the row's threads. A thread holds N pairs, 16 bytes of each
 // half; D = 64, 32 + 2 * 4 head rows of bfloat16: 10 KB a token moved.
-// Measured: 16721 such tokens (172 MB) 32.4 us, 5.3 TB/s; one token 2.2 us.
+// Measured: 16721 such tokens (172 MB) 32.1 us, 5.4 TB/s; one token 1.8 us.
 template <typename TI, typename TC, int D>
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int N = 16 / sizeof(TI), LANES = D / 2 / N;  // pairs of a thread, threads of a row
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
 }
 
 // Rows back as float32 or 16 bits: 16 bytes of output a thread and row.
-// Measured: 32593 tokens of 8 heads of 128 (bfloat16, 267 MB) 45.8 us, 5.8 TB/s.
+// Measured: 32593 tokens of 8 heads of 128 (bfloat16, 267 MB) 45.2 us, 5.9 TB/s.
 template <typename TC, typename TO, int D>
 __global__ void __launch_bounds__(kThreads)
     read_kernel(const __grid_constant__ PagedView c, const int32_t* seq, const int32_t* pos, int32_t tokens,
