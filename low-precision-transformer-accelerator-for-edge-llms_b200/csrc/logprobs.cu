@@ -37,11 +37,11 @@ namespace {
 constexpr int kUnroll = 4;        // 16-byte pieces of a thread in a tile
 constexpr int kTile = kUnroll * 32, kTileBytes = kTile * 16;  // pieces and bytes of a warp's tile
 // Tiles of a warp under way, warps of a CTA that sum rows, that put results
-// together, and such CTAs an SM holds. 2048 rows of 32000 float32 take 47.8 us
-// (5.5 TB/s) with 2, 8, 2, 3; with four tiles under way 54.9 (SMs drift apart:
-// the rows are handed out beforehand), with one result warp 65.5, with two
-// CTAs of 8 + 2 or 8 + 4 warps 50.9 and 51.2, and 52 to 57 where all warps of
-// a CTA work on the results between rows.
+// together, and such CTAs an SM holds. 2048 rows of 32000 float32 took 47.8 us
+// with 2, 8, 2, 3 (now 49.4, 5.3 TB/s); with four tiles under way 54.9 (SMs
+// drift apart: the rows are handed out beforehand), with one result warp 65.5,
+// with two CTAs of 8 + 2 or 8 + 4 warps 50.9 and 51.2, and 52 to 57 where all
+// warps of a CTA work on the results between rows.
 constexpr int kStages = 2;
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kPostWarps = 2;

@@ -171,9 +171,9 @@ struct Shape {
   // Tiles of a warp under way and CTAs an SM holds, each against the time of
   // the kernel as it was then. One context of 131149 positions (bf16, heads of
   // 128), 96.5 us: 3 tiles 151 (one CTA fits), 3 CTAs 129 (168 registers spill).
-  // 64 contexts up to 2048 over INT8 heads of 64, 20.4 us: 4 tiles and 2 CTAs
-  // 23.8, 4 CTAs 20.8 (256 contexts: 46.5, 49.5). Tiles of 16 positions take
-  // 62 us there.
+  // 64 contexts up to 2048 over INT8 heads of 64, 18.7 us: 3 tiles 19.1; when
+  // it took 20.4, 4 tiles and 2 CTAs 23.8, 4 CTAs 20.8 (256 contexts: 46.5, 49.5;
+  // 62 with tiles of 16 positions).
   static constexpr int STAGES = 2;
   static constexpr int CTAS = MT == 1 && RB == 64 ? 3 : 2;
   // Shared memory: rings, the warps' partial results, the query's parts, then
