@@ -97,7 +97,7 @@ def _out(name, t, like, shape, dtype):
     if t is None:
         if like.dtype is dtype and like.shape == shape:
             return torch.empty_like(like, memory_format=torch.contiguous_format)
-        return like.new_empty(shape, dtype=dtype)
+        return like.new_empty(*shape, dtype=dtype)  # (sizes one by one: 0.4 us less than a tuple)
     if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == like.device
             and t.is_contiguous() and not t.data_ptr() & 15):
         raise _bad(name, t, f"a contiguous {dtype} {list(shape)} tensor on {like.device}, 16-byte aligned")
@@ -351,7 +351,7 @@ def token_logprobs(logits, tokens=None, top_k: int = 0) -> TokenLogprobs:
     else:
         lp, ent, top = logits.new_empty(n * (2 + top_k), dtype=f32).split_with_sizes((n, n, n * top_k))
     top = top.view(n, top_k)
-    ids = logits.new_empty((n, top_k), dtype=torch.int32)
+    ids = logits.new_empty(n, top_k, dtype=_INT32)
     if n:
         _enqueue("tl_token_logprobs", load_library().tl_token_logprobs, gpu,
                  _LOGPROBS.pack(logits.data_ptr(), tp, 0 if lp is None else lp.data_ptr(), ent.data_ptr(),
