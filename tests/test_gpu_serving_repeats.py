@@ -40,3 +40,41 @@ def test_attend_repeat(pkg, cache, heads, kv_heads, d, page):
     lengths = i32(lens)
     assert differing(lambda: c.attend(q, table, lengths, return_lse=True), 3000) == 0
     pkg.shim.check(pkg.load_library().tl_device_error(), "tl_device_error")
+
+
+@pytest.mark.parametrize("cache,rows,heads,kv_heads,d,page", [(I8, 64, 32, 4, 64, 16), (BF16, 3, 32, 8, 128, 48)],
+                         ids=str)
+def test_calls_in_a_row(pkg, cache, rows, heads, kv_heads, d, page):
+    """A step's calls placed behind one another as the stream takes them give what they give with the GPU idle
+    between them (each call's blocks may be there before the call before has ended)."""
+    steps, context = 100, 500
+    pages = -(-(context + steps) // page)
+    table = torch.randperm(rows * pages, generator=gen(21), device="cuda").to(torch.int32).view(rows, pages)
+    cos, sin = (torch.from_numpy(t).cuda() for t in pkg.rope_tables(context + steps, d, 10000.0))
+    seq = torch.arange(rows, dtype=torch.int32, device="cuda")
+    prompt = torch.randn((rows * context, kv_heads, d), generator=gen(22), device="cuda")
+    qkv = torch.randn((steps, rows, heads + 2 * kv_heads, d), generator=gen(23), device="cuda")
+    pos = torch.arange(context, context + steps, dtype=torch.int32, device="cuda")[:, None].repeat(1, rows)
+    lengths = pos + 1
+
+    def run(idle):
+        c = pkg.PagedKVCache(rows * pages, page, kv_heads, d, cache)
+        at = torch.arange(context, dtype=torch.int32, device="cuda").repeat(rows)
+        c.append(prompt, prompt, table, seq.repeat_interleave(context), at, cos, sin)
+        q = torch.empty((rows, heads, d), device="cuda")
+        out, lse = torch.empty((steps, rows, heads, d), device="cuda"), torch.empty((steps, rows, heads), device="cuda")
+        k, v = (torch.empty((steps, rows, kv_heads, d), device="cuda") for _ in range(2))
+        for i in range(steps):
+            x = qkv[i]
+            c.append(x[:, heads:heads + kv_heads], x[:, heads + kv_heads:], table, seq, pos[i], cos, sin, q=x[:, :heads],
+                     q_out=q)
+            idle()
+            c.attend(q, table, lengths[i], out=out[i], lse=lse[i])
+            idle()
+            c.read(table, seq, pos[i], k_out=k[i], v_out=v[i])
+            idle()
+        return out, lse, k, v
+
+    want = run(torch.cuda.synchronize)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(run(lambda: None), want))
