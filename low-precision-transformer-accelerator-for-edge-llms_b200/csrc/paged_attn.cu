@@ -19,6 +19,10 @@
 //    has few rows, so a 128-row tcgen05 tile would be mostly padding and its
 //    result would have to come back through tensor memory; the 16-row tile is
 //    small enough to stay below the issue limit at full bandwidth.
+// Measured: one context of 131149 positions (bf16, 8 kv heads of 128) 90.3 us,
+// 5.9 TB/s; 16 contexts up to 8192 (float16) 50.7 us, 5.4 TB/s; 64 up to 2048
+// over INT8 (4 kv heads of 64) 18.6 us, 2.0 TB/s: 38 MB are too few to hide the
+// start (4 us), the joins (3 us) and the rounds' own chain (1.6 us each).
 //
 // Precision. Keys and values are exact, the other operand is split so that
 // nothing but its last bits is rounded; accumulators, maxima and sums are
