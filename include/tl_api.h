@@ -619,7 +619,7 @@ TL_API tl_status tl_paged_read(const tl_paged_kv* cache, const tl_paged_read_arg
  * multiple of kv_heads. Sums and softmax statistics are float32; products run
  * on the tensor cores with the query and the probabilities split into parts of
  * fewer bits that add up to at least 22 of a float32 query's 24 bits (counted
- * from its row's largest element) and 16 (TL_BF16) or 22 of a probability's.
+ * from its row's largest element) and 24 (TL_BF16) or 22 of a probability's.
  * workspace: tl_paged_attn_workspace_bytes bytes of device memory, 16-byte
  * aligned, zeroed once by the caller before its first call; every call leaves
  * it ready for the next. Calls that share one workspace must not overlap on the GPU. The call

@@ -31,8 +31,12 @@
 //    query (or of its probabilities), row g + 8 the low part, what rounding
 //    the high part to 16 bits left over. The sum of the two rows of the
 //    product is the product with a 22-bit (float16) or 16-bit (bf16) operand,
-//    for no more instructions than one part takes with <= 8 heads. For a
-//    float32 query over a bf16 pool a third part (24 bits) takes a second MMA.
+//    for no more instructions than one part takes with <= 8 heads. Over a bf16
+//    pool a third part (24 bits) takes a second MMA: of the query where it is
+//    float32, of the probabilities always. With 16 bits of those, 15 and 26 of
+//    10000 bfloat16 outputs (17 and 5000 positions) were not the rounded
+//    float64 result, with 24 bits 1 and 7; one context of 131149 positions
+//    takes the same 89 us, 64 up to 2048 (4 kv heads of 64) 20.8 for 19.9.
 //  * Over an INT8 pool the query is a 22-bit integer times a power of two, as
 //    three signed digits to the base 256: two in the tile's rows, the third by
 //    a second MMA. Their sums are whole numbers. The probabilities are split as
@@ -184,6 +188,7 @@ struct Shape {
   // scales (int8), tile masks, partial m and l, query scales, barriers.
   static constexpr int RING = kWarps * STAGES * STAGE;
   static constexpr bool THIRD = I8 || PARTS == 3;       // the query has a third part
+  static constexpr bool PTHIRD = BF;                    // the probabilities have a third part
   static constexpr int QROW = I8 ? D : D * 2;           // bytes of a part of a head's query
   static constexpr int QTILE = 16 * QROW, QTHIRD = THIRD ? 8 * QROW : 0;
   static constexpr int PARTS_AT = RING;
@@ -877,7 +882,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
         }
         // ---- probabilities, high and low rows
         uint32_t pa[MT][KT / 16][4];
-        uint32_t pc[S::PARTS == 3 ? MT : 1][KT / 16][2];
+        uint32_t pc[S::PTHIRD ? MT : 1][KT / 16][2];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           const float ref = m[mt] == -INFINITY ? 0.0f : m[mt];
@@ -892,7 +897,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
             }
             pa[mt][j >> 1][2 * (j & 1)] = split<S::BF>(x, y);
             pa[mt][j >> 1][2 * (j & 1) + 1] = split<S::BF>(x, y);
-            if constexpr (S::PARTS == 3) pc[mt][j >> 1][j & 1] = split<S::BF>(x, y);
+            if constexpr (S::PTHIRD) pc[mt][j >> 1][j & 1] = split<S::BF>(x, y);
           }
         }
         // ---- o += p v
@@ -900,8 +905,8 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
             mma16<S::BF>(o[mt][n], pa[mt][kk], b0, b1);
-            if constexpr (S::PARTS == 3) {
-              const uint32_t third[4] = {pc[mt][kk][0], 0u, pc[mt][kk][1], 0u};
+            if constexpr (S::PTHIRD) {
+              const uint32_t third[4] = {0u, pc[mt][kk][0], 0u, pc[mt][kk][1]};
               mma16<S::BF>(o[mt][n], third, b0, b1);
             }
           }
@@ -1083,8 +1088,8 @@ tl_status attend_launch(AttendArgs& a, cudaStream_t s) {
 
 // Groups of up to 8 query heads fit one 16-row tile, larger ones take two at a
 // time so that the pool is read once for every 16 heads: groups of 16 over one
-// context of 131149 positions (bf16, heads of 128) 74 us, 89 with one tile; 64
-// contexts up to 8192 over INT8 heads of 64, 63 and 72. INT8 heads of 128 take
+// context of 131149 positions (bf16, 4 kv heads of 128) 82 us, 90 with one tile;
+// 64 contexts up to 8192 over INT8 (4 kv heads of 64) 64 and 73. INT8 heads of 128 take
 // one tile at a time: two spill registers, 53 us against 43 (64 contexts up to
 // 2048), 152 against 132 (256 of them).
 template <int POOL, int D, int PARTS>
