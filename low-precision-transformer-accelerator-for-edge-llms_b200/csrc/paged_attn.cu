@@ -36,7 +36,7 @@
 //    float32, of the probabilities always. With 16 bits of those, 15 and 26 of
 //    10000 bfloat16 outputs (17 and 5000 positions) were not the rounded
 //    float64 result, with 24 bits 1 and 7; one context of 131149 positions
-//    takes the same 89 us, 64 up to 2048 (4 kv heads of 64) 20.8 for 19.9.
+//    takes the same 89 us, 64 up to 2048 (4 kv heads of 64) 21.2 for 19.9.
 //  * Over an INT8 pool the query is a 22-bit integer times a power of two, as
 //    three signed digits to the base 256: two in the tile's rows, the third by
 //    a second MMA. Their sums are whole numbers. The probabilities are split as
@@ -152,6 +152,22 @@ TL_DEV uint32_t split(float& x, float& y) {
     return *reinterpret_cast<const uint32_t*>(&h);
   }
 }
+
+// Half of two bfloat16 values (exact), or the values: where a third part has an
+// MMA of its own, both MMAs take half of the high part. Rows of zeros there
+// would make a NaN of an infinite element.
+template <bool HALF>
+TL_DEV uint32_t half(uint32_t x) {
+  if constexpr (!HALF) return x;
+  const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), __float2bfloat162_rn(0.5f));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// Sum of the products with the high and with the low parts. An infinity among
+// the stored elements (a float16 pool holds what append rounds to one) makes
+// the first the whole answer, infinite by the sign of the operand, and the
+// second a NaN or an infinity by the sign of what rounding left over.
+TL_DEV float add_parts(float hi, float lo) { return fabsf(hi) < INFINITY ? hi + lo : hi; }
 
 // Two int8 values, biased by 128 and placed in the low bytes of two float16
 // 0x64xx = 1024 + byte, minus 1152: exact.
@@ -547,26 +563,26 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
     }
     // the scale's sign goes into the query, so that larger products are larger scores
     float f = copysignf(1.0f, a.scale), back = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);
+    float top = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < kQ; ++e) {
+      top = fmaxf(top, fabsf(x[e]));
+      bad |= !(fabsf(x[e]) < INFINITY);
+    }
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) {
+      if (!S::BF) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+    }
     if constexpr (!S::BF) {
       // a power of two that takes the row's largest element to [2^10, 2^11), or [2^21, 2^22) for int8 digits
-      float top = 0.0f;
-      bool bad = false;
-#pragma unroll
-      for (int e = 0; e < kQ; ++e) {
-        top = fmaxf(top, fabsf(x[e]));
-        bad |= !(fabsf(x[e]) < INFINITY);
-      }
-#pragma unroll
-      for (int o = 1; o < kLanes; o <<= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        bad |= __shfl_xor_sync(0xffffffffu, bad, o);
-      }
       constexpr int kTop = S::I8 ? 21 : 10;
       const int sh = max(-120, min(120, kTop - (static_cast<int>(__float_as_uint(top) >> 23) - 127)));
       f *= __int_as_float((127 + sh) << 23);
       back *= __int_as_float((127 - sh) << 23);
-      if (bad) back = __int_as_float(0x7fc00000);  // a NaN or an infinity in the query makes the row NaN
     }
+    if (bad) back = __int_as_float(0x7fc00000);  // a NaN or an infinity in the query makes the row NaN
     if (qd == 0) reinterpret_cast<float*>(smem + S::QSCALE)[qh] = back;
     unsigned char* tile = smem + S::QUERY + (qh >> 3) * (S::QTILE + S::QTHIRD);
     const int row = qh & 7;
@@ -594,7 +610,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
       for (int e = 0; e < kQ; e += 2) {
         const int d = qd + e, at = (((d >> 3) ^ row) << 4) + (d & 7) * 2;  // 16-byte pieces turned by the row
         float u = x[e] * f, v = x[e + 1] * f;
-        *reinterpret_cast<uint32_t*>(tile + row * S::QROW + at) = split<S::BF>(u, v);
+        *reinterpret_cast<uint32_t*>(tile + row * S::QROW + at) = half<S::PARTS == 3>(split<S::BF>(u, v));
         *reinterpret_cast<uint32_t*>(tile + (row + 8) * S::QROW + at) = split<S::BF>(u, v);
         if constexpr (S::PARTS == 3)
           *reinterpret_cast<uint32_t*>(tile + S::QTILE + row * S::QROW + at) = split<S::BF>(u, v);
@@ -807,8 +823,9 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
                   const uint32_t b0 = k ? w[j].z : w[j].x, b1 = k ? w[j].w : w[j].y;
                   mma16<S::BF>(c[j][mt], qa[mt][2 * q + k], b0, b1);
                   if constexpr (S::PARTS == 3) {
-                    const uint32_t low[4] = {third[mt][2 * q + k][0], 0u, third[mt][2 * q + k][1], 0u};
-                    mma16<S::BF>(c[j][mt], low, b0, b1);
+                    const uint32_t* high = qa[mt][2 * q + k];
+                    const uint32_t rest[4] = {high[0], third[mt][2 * q + k][0], high[2], third[mt][2 * q + k][1]};
+                    mma16<S::BF>(c[j][mt], rest, b0, b1);
                   }
                 }
             }
@@ -817,8 +834,8 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
           for (int j = 0; j < KT / 8; ++j)
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              s[mt][j][0] = c[j][mt][0] + c[j][mt][2];
-              s[mt][j][1] = c[j][mt][1] + c[j][mt][3];
+              s[mt][j][0] = add_parts(c[j][mt][0], c[j][mt][2]);
+              s[mt][j][1] = add_parts(c[j][mt][1], c[j][mt][3]);
             }
         }
         if (live != full)
@@ -895,7 +912,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
               x *= vs[j][0] * vinv;
               y *= vs[j][1] * vinv;
             }
-            pa[mt][j >> 1][2 * (j & 1)] = split<S::BF>(x, y);
+            pa[mt][j >> 1][2 * (j & 1)] = half<S::PTHIRD>(split<S::BF>(x, y));
             pa[mt][j >> 1][2 * (j & 1) + 1] = split<S::BF>(x, y);
             if constexpr (S::PTHIRD) pc[mt][j >> 1][j & 1] = split<S::BF>(x, y);
           }
@@ -906,8 +923,8 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
           for (int mt = 0; mt < MT; ++mt) {
             mma16<S::BF>(o[mt][n], pa[mt][kk], b0, b1);
             if constexpr (S::PTHIRD) {
-              const uint32_t third[4] = {0u, pc[mt][kk][0], 0u, pc[mt][kk][1]};
-              mma16<S::BF>(o[mt][n], third, b0, b1);
+              const uint32_t rest[4] = {pa[mt][kk][0], pc[mt][kk][0], pa[mt][kk][2], pc[mt][kk][1]};
+              mma16<S::BF>(o[mt][n], rest, b0, b1);
             }
           }
         };
@@ -967,14 +984,14 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
         for (int n = 0; n < D / 8; n += S::I8 ? 2 : 1) {
           if constexpr (S::I8) {
             float4 v;
-            v.x = (o[mt][n][0] + o[mt][n][2]) * vback;
-            v.y = (o[mt][n + 1][0] + o[mt][n + 1][2]) * vback;
-            v.z = (o[mt][n][1] + o[mt][n][3]) * vback;
-            v.w = (o[mt][n + 1][1] + o[mt][n + 1][3]) * vback;
+            v.x = add_parts(o[mt][n][0], o[mt][n][2]) * vback;
+            v.y = add_parts(o[mt][n + 1][0], o[mt][n + 1][2]) * vback;
+            v.z = add_parts(o[mt][n][1], o[mt][n][3]) * vback;
+            v.w = add_parts(o[mt][n + 1][1], o[mt][n + 1][3]) * vback;
             *reinterpret_cast<float4*>(row + ((8 * n + 4 * t) ^ turn)) = v;
           } else {
             *reinterpret_cast<float2*>(row + ((8 * n + 2 * t) ^ turn)) =
-                make_float2(o[mt][n][0] + o[mt][n][2], o[mt][n][1] + o[mt][n][3]);
+                make_float2(add_parts(o[mt][n][0], o[mt][n][2]), add_parts(o[mt][n][1], o[mt][n][3]));
           }
         }
       }
@@ -1088,7 +1105,7 @@ tl_status attend_launch(AttendArgs& a, cudaStream_t s) {
 
 // Groups of up to 8 query heads fit one 16-row tile, larger ones take two at a
 // time so that the pool is read once for every 16 heads: groups of 16 over one
-// context of 131149 positions (bf16, 4 kv heads of 128) 82 us, 90 with one tile;
+// context of 131149 positions (bf16, 4 kv heads of 128) 85 us, 90 with one tile;
 // 64 contexts up to 8192 over INT8 (4 kv heads of 64) 64 and 73. INT8 heads of 128 take
 // one tile at a time: two spill registers, 53 us against 43 (64 contexts up to
 // 2048), 152 against 132 (256 of them).
