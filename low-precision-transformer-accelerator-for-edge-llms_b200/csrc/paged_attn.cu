@@ -562,7 +562,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
                                     : __half2float(__ushort_as_half(static_cast<unsigned short>(half)));
     }
     // the scale's sign goes into the query, so that larger products are larger scores
-    float f = copysignf(1.0f, a.scale), back = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);
+    float f = copysignf(1.0f, a.scale), back = fabsf(a.scale) * kLog2e;
     float top = 0.0f;
     bool bad = false;
 #pragma unroll
@@ -582,6 +582,10 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
       f *= __int_as_float((127 + sh) << 23);
       back *= __int_as_float((127 - sh) << 23);
     }
+    // not 0 (a scale of 0, or one that underflows with a small query): times it, -infinity stays what it is and
+    // every finite product is below 1e-6; a NaN passes
+    const float least = __int_as_float(1);
+    back = back < least ? least : back;
     if (bad) back = __int_as_float(0x7fc00000);  // a NaN or an infinity in the query makes the row NaN
     if (qd == 0) reinterpret_cast<float*>(smem + S::QSCALE)[qh] = back;
     unsigned char* tile = smem + S::QUERY + (qh >> 3) * (S::QTILE + S::QTHIRD);
