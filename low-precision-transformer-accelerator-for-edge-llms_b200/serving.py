@@ -115,6 +115,13 @@ def _enqueue(what, fn, gpu, *args):
         check(code, what)
 
 
+def _not_captured(device):
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a paged cache cannot be made while the current stream is being captured: what clears "
+                               "its memory would only be recorded")
+
+
 class PagedKVCache:
     """One layer's pool of KV pages (tl_paged_kv).
 
@@ -130,7 +137,9 @@ class PagedKVCache:
     one cache are serialized by the caller, as on an engine: on one stream, or
     ordered by events. No call synchronises or allocates beyond its outputs
     (taken from torch's allocator), so with preallocated outputs calls can be
-    captured in a CUDA graph.
+    captured in a CUDA graph, the first one too. Making a cache allocates the
+    attention's scratch (2 to 11 MB), waits until the current stream has cleared
+    it, and is refused (RuntimeError) while that stream is being captured.
     """
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=None, device="cuda"):
@@ -143,6 +152,7 @@ class PagedKVCache:
             raise ValueError(f"num_pages, page_size and kv_heads must be positive and head_dim one of {HEAD_DIMS}")
         if not torch.cuda.is_available():
             raise RuntimeError("no CUDA device visible: the paged cache runs only on the GPU")
+        _not_captured(device)
         shape = (num_pages, kv_heads, page_size, head_dim)
         k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
         ks, vs = ((torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
@@ -152,12 +162,12 @@ class PagedKVCache:
     @classmethod
     def from_tensors(cls, k, v, k_scale=None, v_scale=None) -> "PagedKVCache":
         """A cache over tensors the caller owns (one layer's slice of a larger pool, for instance)."""
+        _need_torch()
         self = cls.__new__(cls)
         self._bind(k, v, k_scale, v_scale)
         return self
 
     def _bind(self, k, v, k_scale, v_scale):
-        _need_torch()
         for name, t in (("k", k), ("v", v)):
             if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 4 and t.dtype in _POOL_CODES
                     and t.numel() and t.is_contiguous() and not t.data_ptr() & 15):
@@ -165,6 +175,7 @@ class PagedKVCache:
                                     "head_dim] of int8, bfloat16 or float16")
         if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
             raise ValueError("k and v must agree in shape, type and device")
+        _not_captured(k.device)
         if k.shape[3] not in HEAD_DIMS:
             raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {k.shape[3]}")
         for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
@@ -184,8 +195,13 @@ class PagedKVCache:
         self._view = PagedView(*ptr, _POOL_CODES[k.dtype], *k.shape)
         self._ref = C.byref(self._view)
         self._scale = self.head_dim ** -0.5
-        self._work = None
-        self._work_bytes = 0
+        # The attention's scratch for any number of heads (its size depends on neither rows nor lengths). The
+        # kernel needs it zeroed before the first call, whichever stream that runs on, and a call that is only
+        # recorded in a graph clears nothing: so it is made here, and there when this returns.
+        self._work_bytes = max(lib.tl_paged_attn_workspace_bytes(self.kv_heads * group, self.kv_heads, self.head_dim)
+                               for group in (1, 16))
+        self._work = torch.zeros(self._work_bytes, dtype=torch.uint8, device=self.device)
+        torch.cuda.current_stream(self.device).synchronize()
 
     # ---------------------------------------------------------------- calls
     def _table(self, t):
@@ -293,26 +309,11 @@ class PagedKVCache:
         if return_lse or lse is not None:
             lse = _out("lse", lse, q, (n, heads), torch.float32)
         if n:
-            work = self._workspace(heads)
             _enqueue("tl_paged_attn_decode", self._attend, gpu, self._ref,
-                     _ATTEND.pack(qp, sp, lp, tp, out.data_ptr(), 0 if lse is None else lse.data_ptr(), work,
-                                  self._work_bytes, qs, ts, _FLOAT_CODES[dt], seqs, pages, n, heads,
-                                  self._scale if sm_scale is None else sm_scale))
+                     _ATTEND.pack(qp, sp, lp, tp, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                                  self._work.data_ptr(), self._work_bytes, qs, ts, _FLOAT_CODES[dt], seqs, pages, n,
+                                  heads, self._scale if sm_scale is None else sm_scale))
         return (out, lse) if return_lse else out
-
-    def _workspace(self, heads):
-        """The cache's own scratch, allocated at the first call with so many heads
-        (make that call before capturing a graph) and kept: its size does not
-        depend on rows or lengths."""
-        if self._work is None or self._work[1] < heads:
-            need = self._lib.tl_paged_attn_workspace_bytes(heads, self.kv_heads, self.head_dim)
-            kept = self._work  # a larger one may follow while calls that use this one are in flight
-            if need > self._work_bytes:
-                t = torch.zeros(need, dtype=torch.uint8, device=self.device)
-                self._work, self._work_bytes = (t, heads, kept), need
-            else:
-                self._work = (kept[0], heads, kept[2])
-        return self._work[0].data_ptr()
 
 
 class TokenLogprobs(NamedTuple):

@@ -4,7 +4,7 @@ import math
 
 import pytest
 
-from test_gpu_serving import BF16, F16, F32, I8, U, TINY, gen, gpu, i32, pool, u  # noqa: F401 (gpu: the module's fixture)
+from test_gpu_serving import BF16, F16, F32, I8, TINY, U, gen, gpu, i32, pool, u  # noqa: F401 (gpu: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -48,7 +48,8 @@ def rows_of(c, table, n, page):
 
 @pytest.mark.parametrize("cache", [BF16, F16], ids=str)
 @pytest.mark.parametrize("qt", [F32, BF16, F16], ids=str)
-@pytest.mark.parametrize("n,heads,kv_heads,d,page", [(70, 8, 1, 64, 16), (70, 32, 2, 128, 24), (9000, 16, 1, 128, 32), (3, 4, 4, 64, 7)])
+@pytest.mark.parametrize("n,heads,kv_heads,d,page", [(70, 8, 1, 64, 16), (70, 32, 2, 128, 24), (9000, 16, 1, 128, 32),
+                                                      (3, 4, 4, 64, 7)])
 def test_infinite_keys_and_values(pkg, cache, qt, n, heads, kv_heads, d, page):
     """An infinite key element scores its position +-infinity by the query's sign there; an infinite value element makes
     its column +-infinity, and NaN where both signs meet."""
