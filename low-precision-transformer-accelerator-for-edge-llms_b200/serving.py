@@ -135,11 +135,14 @@ class PagedKVCache:
     device). Entries that name no sequence, position or page are skipped (see
     each call), so a batch of fixed size is padded with ``seq = -1``. Calls on
     one cache are serialized by the caller, as on an engine: on one stream, or
-    ordered by events. No call synchronises or allocates beyond its outputs
-    (taken from torch's allocator), so with preallocated outputs calls can be
-    captured in a CUDA graph, the first one too. Making a cache allocates the
-    attention's scratch (2 to 11 MB), waits until the current stream has cleared
-    it, and is refused (RuntimeError) while that stream is being captured.
+    ordered by events. A cache may be dropped while its calls run on whichever
+    stream: what it has allocated is kept until they end (tensors that the caller
+    passed are the caller's to keep, and a cache lives as long as a graph with its
+    calls). No call synchronises or allocates beyond its outputs (taken from
+    torch's allocator), so with preallocated outputs calls can be captured in a
+    CUDA graph, the first one too. Making a cache allocates the attention's
+    scratch (2 to 11 MB), waits until the current stream has cleared it, and is
+    refused (RuntimeError) while that stream is being captured.
     """
 
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=None, device="cuda"):
@@ -158,6 +161,7 @@ class PagedKVCache:
         ks, vs = ((torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
                   if dtype == torch.int8 else (None, None))
         self._bind(k, v, ks, vs)
+        self._owned += [t for t in (k, v, ks, vs) if t is not None]
 
     @classmethod
     def from_tensors(cls, k, v, k_scale=None, v_scale=None) -> "PagedKVCache":
@@ -202,6 +206,15 @@ class PagedKVCache:
                                for group in (1, 16))
         self._work = torch.zeros(self._work_bytes, dtype=torch.uint8, device=self.device)
         torch.cuda.current_stream(self.device).synchronize()
+        self._owned = [self._work]
+        self._streams = {_stream(self._gpu)}  # raw handles of the streams that the allocator knows to use them
+
+    def _enter_stream(self):
+        """The current stream's first call: without this the allocator would hand the memory on as soon as the cache
+        is dropped, ordered behind the stream that it was allocated on only."""
+        for t in self._owned:
+            t.record_stream(torch.cuda.current_stream(self.device))
+        self._streams.add(_stream(self._gpu))
 
     # ---------------------------------------------------------------- calls
     def _table(self, t):
@@ -254,6 +267,8 @@ class PagedKVCache:
         elif q_out is not None:
             raise ValueError("q_out without q")
         if n:
+            if _stream(gpu) not in self._streams:
+                self._enter_stream()
             _enqueue("tl_paged_append", self._append, gpu, self._ref,
                      _APPEND.pack(qp, kp, vp, op, sp, pp, tp, cp, np, qs, ks, vs, ts, _FLOAT_CODES[dt], seqs, pages,
                                   angles, n, heads))
@@ -274,6 +289,8 @@ class PagedKVCache:
         shape = (n, self.kv_heads, self.head_dim)
         k, v = _out("k_out", k_out, self.k, shape, dtype), _out("v_out", v_out, self.k, shape, dtype)
         if n:
+            if _stream(gpu) not in self._streams:
+                self._enter_stream()
             _enqueue("tl_paged_read", self._read, gpu, self._ref,
                      _READ.pack(sp, pp, tp, k.data_ptr(), v.data_ptr(), ts, seqs, pages, n, _FLOAT_CODES[dtype]))
         return k, v
@@ -309,6 +326,8 @@ class PagedKVCache:
         if return_lse or lse is not None:
             lse = _out("lse", lse, q, (n, heads), torch.float32)
         if n:
+            if _stream(gpu) not in self._streams:
+                self._enter_stream()
             _enqueue("tl_paged_attn_decode", self._attend, gpu, self._ref,
                      _ATTEND.pack(qp, sp, lp, tp, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
                                   self._work.data_ptr(), self._work_bytes, qs, ts, _FLOAT_CODES[dt], seqs, pages, n,
