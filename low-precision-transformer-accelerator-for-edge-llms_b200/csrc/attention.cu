@@ -1664,13 +1664,14 @@ cudaError_t attn_prepare() {
 }
 
 cudaError_t attn_read_error(unsigned int* code) {
+  *code = 0;
   for (const void* sym : {static_cast<const void*>(&g_attn_error), static_cast<const void*>(&g_apf_error)}) {
-    cudaError_t e = cudaMemcpyFromSymbol(code, sym, sizeof(unsigned int));
+    unsigned int c = 0;
+    const unsigned int zero = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&c, sym, sizeof(unsigned int));
+    if (e == cudaSuccess && c) e = cudaMemcpyToSymbol(sym, &zero, sizeof(unsigned int));
     if (e != cudaSuccess) return e;
-    if (*code) {
-      unsigned int zero = 0;
-      return cudaMemcpyToSymbol(sym, &zero, sizeof(unsigned int));
-    }
+    if (*code == 0) *code = c;
   }
   return cudaSuccess;
 }

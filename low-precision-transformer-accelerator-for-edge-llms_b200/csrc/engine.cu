@@ -1053,7 +1053,7 @@ tl_status run_decode_loop(tl_engine* e, int M, int budget, bool* aborted) {
     if (!any) break;
   }
   unsigned int code = 0;
-  TL_CU(tc_read_error(&code));
+  TL_CU(engine_read_error(&code));
   if (code) {
     g_last_error = "device wait expired (code " + std::to_string(code) + ", detail " +
                    std::to_string(decode1_last_detail()) + ")";
@@ -1960,7 +1960,7 @@ tl_status tl_synchronize(tl_engine* e) {
   TL_CU(cudaStreamSynchronize(e->stream));
   TL_CU(cudaGetLastError());
   unsigned int code = 0;
-  TL_CU(tc_read_error(&code));
+  TL_CU(engine_read_error(&code));
   if (code) {
     g_last_error = "device wait expired (code " + std::to_string(code) + ", detail " +
                    std::to_string(decode1_last_detail()) + ")";

@@ -1088,21 +1088,11 @@ cudaError_t prepare_tc() {
   return prepare_tcp();
 }
 
-// Reads and clears the bounded-wait error words of the tcgen05 GEMM, the
-// attention kernels, the persistent decode step and the tensor-parallel
-// exchange (0 = none expired).
 cudaError_t tc_read_error(unsigned int* code) {
   cudaError_t e = cudaMemcpyFromSymbol(code, g_tc_error, sizeof(unsigned int));
-  if (e != cudaSuccess) return e;
-  if (*code) {
-    unsigned int zero = 0;
-    return cudaMemcpyToSymbol(g_tc_error, &zero, sizeof(unsigned int));
-  }
-  e = attn_read_error(code);
-  if (e != cudaSuccess || *code) return e;
-  e = decode1_read_error(code);
-  if (e != cudaSuccess || *code) return e;
-  return tp_read_error(code);
+  if (e != cudaSuccess || !*code) return e;
+  unsigned int zero = 0;
+  return cudaMemcpyToSymbol(g_tc_error, &zero, sizeof(unsigned int));
 }
 
 }  // namespace tl

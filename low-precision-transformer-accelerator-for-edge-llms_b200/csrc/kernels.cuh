@@ -103,9 +103,27 @@ cudaError_t launch_gemm_tc(const TcPlan& p, const TcArgs& a, cudaStream_t s, boo
 cudaError_t prepare_tc();
 int tc_max_stages(int bn, int ks = 1);
 int tc_pick_bn(int M);
-// Reads (and clears) the device error word of the tensor-core kernels: 0 ok,
+// Reads (and clears) the device error word of the tensor-core GEMMs: 0 ok,
 // else the code of the bounded wait that expired.
 cudaError_t tc_read_error(unsigned int* code);
+// Reads and clears the words of all `readers`, whatever the others hold (one
+// that stayed behind would be reported for later work): the first that is set
+// is the code, the first failure the result.
+template <size_t N>
+cudaError_t read_errors(cudaError_t (*const (&readers)[N])(unsigned int*), unsigned int* code) {
+  cudaError_t result = cudaSuccess;
+  *code = 0;
+  for (auto* reader : readers) {
+    unsigned int c = 0;
+    const cudaError_t e = reader(&c);
+    if (result == cudaSuccess) result = e;
+    if (*code == 0) *code = c;
+  }
+  return result;
+}
+// The words of everything an engine runs: tensor-core GEMMs, attention, the
+// persistent decode step and the tensor-parallel exchange (ops.cu).
+cudaError_t engine_read_error(unsigned int* code);
 int device_sm_count();
 
 // ---- persistent single-sequence decode step (decode1.cu)

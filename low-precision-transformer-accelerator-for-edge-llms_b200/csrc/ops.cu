@@ -32,14 +32,17 @@ tl_status check_gemm(const void* a, const void* w, int M, int N, int K) {
 
 }  // namespace
 
+cudaError_t tl::engine_read_error(unsigned int* code) {
+  return read_errors({tc_read_error, attn_read_error, decode1_read_error, tp_read_error}, code);
+}
+
 extern "C" {
 
 tl_status tl_device_error(void) {
   unsigned int code = 0;
   if (cudaDeviceSynchronize() != cudaSuccess) return TL_ERR_CUDA;
-  if (tc_read_error(&code) != cudaSuccess) return TL_ERR_CUDA;
-  if (code == 0 && paged_attn_read_error(&code) != cudaSuccess) return TL_ERR_CUDA;
-  if (code == 0 && logprob_read_error(&code) != cudaSuccess) return TL_ERR_CUDA;
+  if (read_errors({engine_read_error, paged_attn_read_error, logprob_read_error}, &code) != cudaSuccess)
+    return TL_ERR_CUDA;
   return code ? TL_ERR_TIMEOUT : TL_OK;
 }
 
