@@ -662,7 +662,8 @@ TL_API tl_status tl_paged_attn_decode(const tl_paged_kv* cache, const tl_paged_a
  * no token: logprob 0 (a sum over a padded batch skips it); tokens[r] >= vocab
  * gives NaN. A row of -infinity alone has entropy 0 and logprob -infinity. A
  * row with a NaN or +infinity has no distribution: logprob, entropy and
- * top_logprobs are NaN, ids -1. Needs no workspace. */
+ * top_logprobs are NaN, ids -1. Rows of 2^31 - 2^17 bytes and more are refused
+ * (TL_ERR_OUT_OF_RANGE). Needs no workspace. */
 #define TL_TOP_K_MAX 32
 typedef struct tl_token_logprobs_args {
   const void* logits;

@@ -710,6 +710,9 @@ extern "C" tl_status tl_token_logprobs(const tl_token_logprobs_args* args, void*
   if (x.top_k < 0 || (x.top_k > 0 && (!x.top_ids || !x.top_logprobs))) return TL_ERR_INVALID_ARGUMENT;
   if (!x.logprob && !x.entropy && !x.top_k) return TL_ERR_INVALID_ARGUMENT;
   if (x.top_k > TL_TOP_K_MAX) return TL_ERR_OUT_OF_RANGE;
+  // bytes and elements of a row are counted in 31 bits, with room for every CTA's next tile behind its end
+  constexpr int64_t kRowBytes = INT32_MAX - static_cast<int64_t>(kMaxCluster) * kWarps * kTileBytes;
+  if (x.vocab > kRowBytes / dtype_bytes(x.dtype)) return TL_ERR_OUT_OF_RANGE;
   const LogprobArgs a{x.logits, x.row_stride, x.tokens,  x.rows,         x.vocab,
                       x.top_k,  x.logprob,    x.entropy, x.top_logprobs, x.top_ids};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
