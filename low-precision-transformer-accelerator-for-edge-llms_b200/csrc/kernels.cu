@@ -14,6 +14,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 #include <cmath>
 #include <cstdio>
@@ -78,7 +79,7 @@ constexpr int kGemvThreads = 256;
 constexpr int kGemvWarps = kGemvThreads / 32;
 constexpr int kGemvRW = 2;   // weight rows per warp item
 constexpr int kGemvU = 4;    // 16-byte chunks per lane per row per item
-static int g_num_sms[64] = {0};
+static std::atomic<int> g_num_sms[64] = {};  // (any thread's first call sets it)
 
 
 TL_DEV float silu_mul(float g, float u) {
@@ -348,7 +349,7 @@ static NormPlan plan_or_min(int K) {
 static int gemv_grid_x(int N, int MR) {
   int dev = 0;
   cudaGetDevice(&dev);
-  const int sms = (dev >= 0 && dev < 64 && g_num_sms[dev] > 0) ? g_num_sms[dev] : 148;
+  const int sms = (dev >= 0 && dev < 64 && g_num_sms[dev] > 0) ? g_num_sms[dev].load() : 148;
   const int groups = (N + kGemvRW - 1) / kGemvRW;
   const int need = (groups + kGemvWarps - 1) / kGemvWarps;
   // One CTA per SM (8 warps, two work items in flight each) saturates HBM and
@@ -456,8 +457,10 @@ cudaError_t prepare_kernels(int max_k) {
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (max_k <= prepared_k[dev]) return cudaSuccess;
   if (g_num_sms[dev] == 0) {
-    e = cudaDeviceGetAttribute(&g_num_sms[dev], cudaDevAttrMultiProcessorCount, dev);
+    int n = 0;
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
+    g_num_sms[dev] = n;
   }
 #define TL_GEMV_PREP(P, E) \
   if ((e = prepare_gemv_mr<P, E>(max_k)) != cudaSuccess) return e;

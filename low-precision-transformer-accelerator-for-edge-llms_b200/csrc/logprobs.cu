@@ -661,16 +661,12 @@ __global__ void __launch_bounds__(CLUSTER ? kThreads : kThreads + kPostWarps * 3
 
 template <typename T>
 tl_status logprob_launch(const LogprobArgs& a, cudaStream_t s) {
-  static bool ready[64];  // once a device: the rings need more shared memory than the default limit
+  static Once<64> ready;  // the rings need more shared memory than the default limit
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TL_ERR_CUDA;
-  if (!ready[dev]) {
-    const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
-    if (cudaFuncSetAttribute(logprob_kernel<T, false>, attr, kRing) != cudaSuccess ||
-        cudaFuncSetAttribute(logprob_kernel<T, true>, attr, kRing) != cudaSuccess)
-      return TL_ERR_CUDA;
-    ready[dev] = true;
-  }
+  if (cudaGetDevice(&dev) != cudaSuccess || !ready(dev, [] {
+        return allow_shared(logprob_kernel<T, false>, kRing) && allow_shared(logprob_kernel<T, true>, kRing);
+      }))
+    return TL_ERR_CUDA;
   // A row is split over a cluster while there are fewer CTAs than two an SM
   // and every warp has a tile. One row of 32000 float32 over 1, 2, 4, 8 CTAs:
   // 11.9, 8.7, 7.7, 7.7 us; 64 rows of 50021 bfloat16 over 1, 2, 4: 12.0, 9.1,

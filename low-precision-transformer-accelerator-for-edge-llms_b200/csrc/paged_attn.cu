@@ -1087,15 +1087,10 @@ tl_status attend_launch(AttendArgs& a, cudaStream_t s) {
   const int64_t most = static_cast<int64_t>(a.c.hkv) * a.blocks *
                        ((static_cast<int64_t>(a.c.max_pages) * a.c.ps + S::UNIT - 1) / S::UNIT);
   if (most + static_cast<int64_t>(a.c.hkv) * a.blocks * S::GAP > INT32_MAX / a.rows) return TL_ERR_OUT_OF_RANGE;
-  // once a device: the ring needs more shared memory than the default limit
-  static bool ready[64];
+  static Once<64> ready;  // the ring needs more shared memory than the default limit
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TL_ERR_CUDA;
-  if (!ready[dev]) {
-    if (cudaFuncSetAttribute(attend_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess)
-      return TL_ERR_CUDA;
-    ready[dev] = true;
-  }
+  if (cudaGetDevice(&dev) != cudaSuccess || !ready(dev, [] { return allow_shared(attend_kernel<S>, S::SMEM); }))
+    return TL_ERR_CUDA;
   // as many CTAs as the device holds at once, fewer where the table has no room for so many rounds
   const int64_t grid = std::min<int64_t>(most * a.rows, std::min(kMaxCtas, device_sm_count() * S::CTAS));
   a.box = std::gcd(a.c.ps, S::KT);

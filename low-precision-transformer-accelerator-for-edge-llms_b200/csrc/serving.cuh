@@ -8,6 +8,7 @@
 
 #include "../../include/tl_api.h"
 #include "common.cuh"
+#include "once.cuh"
 
 namespace tl {
 
@@ -35,6 +36,11 @@ tl_status launch_serving(void (*kernel)(P...), unsigned grid, int threads, size_
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+// Raises a kernel's limit of dynamic shared memory on the current device.
+template <typename K>
+bool allow_shared(K* kernel, int bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
 }
 // All that the kernels before have written is there; from here on the next one
 // may be placed (not earlier: what it must not overtake has ended by then).
