@@ -58,7 +58,8 @@ def _need_torch():
 
 
 def _bad(name, t, want):
-    got = f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}" if hasattr(t, "dtype") else type(t).__name__
+    got = (f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}" if isinstance(t, _Tensor)
+           else f"{type(t).__module__}.{type(t).__qualname__}")
     return ValueError(f"{name} must be {want}, got {got}")
 
 
@@ -253,7 +254,7 @@ class PagedKVCache:
         if cos is not None or sin is not None:
             if cos is None or sin is None:
                 raise ValueError("cos and sin go together")
-            angles = cos.shape[0]
+            angles = cos.shape[0] if isinstance(cos, torch.Tensor) and cos.dim() else 0
             cp, np = _angles("cos", cos, angles, d, gpu), _angles("sin", sin, angles, d, gpu)
         if q is not None:
             if not angles:
@@ -331,7 +332,7 @@ class PagedKVCache:
             _enqueue("tl_paged_attn_decode", self._attend, gpu, self._ref,
                      _ATTEND.pack(qp, sp, lp, tp, out.data_ptr(), 0 if lse is None else lse.data_ptr(),
                                   self._work.data_ptr(), self._work_bytes, qs, ts, _FLOAT_CODES[dt], seqs, pages, n,
-                                  heads, self._scale if sm_scale is None else sm_scale))
+                                  heads, self._scale if sm_scale is None else float(sm_scale)))
         return (out, lse) if return_lse else out
 
 

@@ -19,7 +19,7 @@ def check(c, calls, want):
     torch.cuda.synchronize()
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
-        for _ in range(40):  # some 20 ms and more of work in front
+        for _ in range(10):  # some 20 ms and more of work in front
             busy @ busy
         got = calls(c)
         end = torch.cuda.Event()
