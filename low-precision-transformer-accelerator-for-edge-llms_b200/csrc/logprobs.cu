@@ -667,10 +667,10 @@ tl_status logprob_launch(const LogprobArgs& a, cudaStream_t s) {
         return allow_shared(logprob_kernel<T, false>, kRing) && allow_shared(logprob_kernel<T, true>, kRing);
       }))
     return TL_ERR_CUDA;
-  // A row is split over a cluster while there are fewer CTAs than two an SM
-  // and every warp has a tile. One row of 32000 float32 over 1, 2, 4, 8 CTAs:
-  // 11.9, 8.7, 7.7, 7.7 us; 64 rows of 50021 bfloat16 over 1, 2, 4: 12.0, 9.1,
-  // 8.6.
+  // A row's CTAs are doubled while the call has no more CTAs than there are SMs and
+  // the row has a tile for every warp of twice as many, four warps aside. One row of
+  // 32000 float32 over 1, 2, 4, 8 CTAs: 11.9, 8.7, 7.7, 7.7 us; 64 rows of 50021
+  // bfloat16 over 1, 2, 4: 12.0, 9.1, 8.6.
   int ctas = 1;
   const int64_t tiles = static_cast<int64_t>(a.vocab) * sizeof(T) / kTileBytes;
   while (ctas < kMaxCluster && static_cast<int64_t>(a.rows) * ctas <= device_sm_count() &&

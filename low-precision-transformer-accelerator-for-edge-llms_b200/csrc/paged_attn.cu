@@ -53,7 +53,11 @@ namespace tl {
 namespace {
 
 constexpr int kWarps = 4;         // warps of a CTA, each on its own tiles
-constexpr int kMaxCtas = 640;     // grid bound (148 SMs x 4 CTAs), sizes the workspace
+// The workspace holds what the CTAs of a full device leave: at most kSms SMs
+// of ctas_per_sm() CTAs, by query heads of a CTA and head_dim.
+constexpr int kSms = 148;
+constexpr int ctas_per_sm(int heads, int d) { return heads == 8 && d == 64 ? 3 : 2; }
+constexpr int kMaxCtas = kSms * 3;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Probabilities are kept as 2^(s' - m) with m 8 below the running maximum, and
@@ -78,7 +82,7 @@ struct AttendArgs {
   float* lse;
   int32_t box;            // rows of a TMA box: the largest that divides a page and a tile
   unsigned int* tickets;  // [kMaxCtas], zero between calls
-  float* records;         // [kMaxCtas][2]: a partial result (HEADS rows, maxima, sums)
+  float* records;         // [CTAs][2]: a partial result (HEADS rows, maxima, sums)
 };
 
 TL_DEV void cp_async16(uint32_t dst, const void* src) {
@@ -200,6 +204,7 @@ struct Shape {
   // 62 with tiles of 16 positions).
   static constexpr int STAGES = 2;
   static constexpr int CTAS = MT == 1 && RB == 64 ? 3 : 2;
+  static_assert(CTAS <= ctas_per_sm(HEADS, D), "sizes the workspace");
   // Shared memory: rings, the warps' partial results, the query's parts, then
   // scales (int8), tile masks, partial m and l, query scales, barriers.
   static constexpr int RING = kWarps * STAGES * STAGE;
@@ -1092,7 +1097,7 @@ tl_status attend_launch(AttendArgs& a, cudaStream_t s) {
   if (cudaGetDevice(&dev) != cudaSuccess || !ready(dev, [] { return allow_shared(attend_kernel<S>, S::SMEM); }))
     return TL_ERR_CUDA;
   // as many CTAs as the device holds at once, fewer where the table has no room for so many rounds
-  const int64_t grid = std::min<int64_t>(most * a.rows, std::min(kMaxCtas, device_sm_count() * S::CTAS));
+  const int64_t grid = std::min<int64_t>(most * a.rows, std::min(kSms, device_sm_count()) * S::CTAS);
   a.box = std::gcd(a.c.ps, S::KT);
   CUtensorMap tm_k, tm_v;
   const long long pool_rows = static_cast<long long>(a.c.pages) * a.c.hkv * a.c.ps;
@@ -1146,8 +1151,9 @@ extern "C" {
 
 size_t tl_paged_attn_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t head_dim) {
   if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
-  const size_t tile = heads / kv_heads <= 8 ? 8 : 16;
-  return kTicketBytes + static_cast<size_t>(kMaxCtas) * 2 * tile * (head_dim + 2) * sizeof(float);
+  const int tile = heads / kv_heads <= 8 ? 8 : 16;
+  return kTicketBytes +
+         static_cast<size_t>(kSms) * ctas_per_sm(tile, head_dim) * 2 * tile * (head_dim + 2) * sizeof(float);
 }
 
 tl_status tl_paged_attn_decode(const tl_paged_kv* cache, const tl_paged_attn_args* args, void* stream) {

@@ -142,7 +142,7 @@ class PagedKVCache:
     calls). No call synchronises or allocates beyond its outputs (taken from
     torch's allocator), so with preallocated outputs calls can be captured in a
     CUDA graph, the first one too. Making a cache allocates the attention's
-    scratch (2 to 11 MB), waits until the current stream has cleared it, and is
+    scratch (2.5 or 5 MB), waits until the current stream has cleared it, and is
     refused (RuntimeError) while that stream is being captured.
     """
 
