@@ -311,6 +311,7 @@ __device__ void join_records(const AttendArgs& a, unsigned char* smem, int4 x) {
     const int h = (tid * 4 + c * kWarps * 128) / D, d = (tid * 4) % D;
     if (h >= nh) return;
     const bool empty = top == -INFINITY && sum == 0.0f;
+    if (empty) v = make_float4(0, 0, 0, 0);  // (weights of 0 may have met an infinite value)
     const float inv = empty ? 0.0f : 1.0f / sum;
     store_out(a.out, a.q_dtype, (head0 + h) * D + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
     if (a.lse && d == 0) a.lse[head0 + h] = empty ? -INFINITY : (top + log2f(sum)) * kLn2;
@@ -1036,6 +1037,7 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
         }
         if (whole) {
           const bool empty = M == -INFINITY && L == 0.0f;
+          if (empty) v = make_float4(0, 0, 0, 0);  // (as when records are joined)
           const float inv = empty ? 0.0f : 1.0f / L;
           store_out(a.out, a.q_dtype, (head0 + h) * D + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
           if (a.lse && d == 0) a.lse[head0 + h] = empty ? -INFINITY : (M + log2f(L)) * kLn2;

@@ -26,6 +26,7 @@ def check(out, lse, q, k, v, scale):
     total = p.sum(-1, keepdim=True)
     none = (total == 0).squeeze(-1)
     want = (p.unsqueeze(-1) * vv).sum(1) / torch.where(total == 0, torch.ones_like(total), total)
+    want[none] = 0
     want_lse = (top + torch.log(total)).squeeze(-1)
     assert torch.equal(lse.double().isnan(), want_lse.isnan())
     fine = want_lse.isfinite()
@@ -90,6 +91,7 @@ def test_position_of_infinite_score_alone(pkg):
         q = torch.randn((1, 8, 64), generator=gen(2), device="cuda")
         q[..., 5] = torch.where(torch.arange(8, device="cuda") % 2 == 0, 1.0, -1.0)
         c.k[table[0, 0], :, 0, 5] = -math.inf
+        c.v[table[0, 0], :, 0, 9] = math.inf
         out, lse = c.attend(q, table, i32([1]), return_lse=True)
         assert torch.all(out[0, ::2] == 0) and torch.all(lse[0, ::2] == -math.inf)
         assert out[0, 1::2].isnan().all() and lse[0, 1::2].isnan().all()
@@ -125,3 +127,18 @@ def test_nonfinite_query(pkg, cache, bad):
     assert torch.equal(out[:, keep], want[:, keep]) and torch.equal(lse[:, keep], want_lse[:, keep])
     assert out[:3, 4].isnan().all() and lse[:3, 4].isnan().all()
     assert torch.all(out[3, 4] == 0) and lse[3, 4] == -math.inf
+
+
+def test_split_row_of_infinite_scores(pkg):
+    """A context over many blocks none of whose positions has weight, some with infinite values."""
+    n = 20000
+    for cache in (BF16, F16):
+        c, table, ref = pool(pkg, [n], 16, 1, 64, cache, 12)
+        q = torch.randn((1, 8, 64), generator=gen(13), device="cuda")
+        q[..., 5] = torch.where(torch.arange(8, device="cuda") % 2 == 0, 1.0, -1.0)
+        pg, off = rows_of(c, table, n, 16)
+        c.k[pg, :, off, 5] = -math.inf
+        c.v[pg[::777], :, off[::777], 9] = math.inf
+        out, lse = c.attend(q, table, i32([n]), return_lse=True)
+        assert torch.all(out[0, ::2] == 0) and torch.all(lse[0, ::2] == -math.inf)
+        assert out[0, 1::2].isnan().all() and lse[0, 1::2].isnan().all()
