@@ -174,7 +174,8 @@ TL_DEV uint32_t half(uint32_t x) {
 TL_DEV float add_parts(float hi, float lo) { return fabsf(hi) < INFINITY ? hi + lo : hi; }
 
 // Two int8 values, biased by 128 and placed in the low bytes of two float16
-// 0x64xx = 1024 + byte, minus 1152: exact.
+// 0x64xx = 1024 + byte, minus 1152: exact (the conversion by a number whose last
+// place is 1: Kim et al., "Who Says Elephants Can't Run", 2022).
 TL_DEV uint32_t bytes_to_half2(uint32_t biased, uint32_t selector) {
   const uint32_t h = __byte_perm(biased, 0x64646464u, selector);
   const uint32_t off = 0x64806480u;
@@ -226,7 +227,8 @@ struct Shape {
   // so that CTAs that cross items get fewer rounds. When the gaps came in, 16
   // contexts up to 8192 (float16, heads of 128) took 61.3 us without them and
   // 54.6, 53.2, 52.0 with 1, 2, 3; 64 up to 2048 over INT8 22.9 and 21.1, 21.8,
-  // 21.7.
+  // 21.7. Rows of 128 bytes, 64 contexts up to 2048, with 1, 2, 3, 4: float16
+  // heads of 64 20.3, 20.1, 20.8, 21.0, INT8 heads of 128 28.4, 28.2, 28.7, 28.8.
   static constexpr int GAP = RB == 256 ? 3 : RB == 128 ? 2 : 1;
   static constexpr int RECORD = HEADS * (D + 2);        // floats of a partial result in the workspace
 };
@@ -646,7 +648,8 @@ __global__ void __launch_bounds__(kWarps * 32, S::CTAS)
     const int pos = (p.rd * kWarps + warp) * KT + lane;
     if (lane >= KT || pos >= p.len) return -1;
     const uint32_t pg = div_page(pos, a.c.div);
-    const int page = __ldg(p.pages + pg);
+    // (no __ldg: the CTA may be there before a kernel that wrote the table has ended)
+    const int page = p.pages[pg];
     if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.c.pages)) return -1;
     return (page * a.c.hkv + p.kvh) * a.c.ps + (pos - static_cast<int>(pg * a.c.div.d));
   };
@@ -1111,7 +1114,7 @@ tl_status attend_launch(AttendArgs& a, cudaStream_t s) {
 
 // Groups of up to 8 query heads fit one 16-row tile, larger ones take two at a
 // time so that the pool is read once for every 16 heads: groups of 16 over one
-// context of 131149 positions (bf16, 4 kv heads of 128) 85 us, 90 with one tile;
+// context of 131149 positions (bf16, 4 kv heads of 128) 84 us, 89 with one tile;
 // 64 contexts up to 8192 over INT8 (4 kv heads of 64) 64 and 73. INT8 heads of 128 take
 // one tile at a time: two spill registers, 53 us against 43 (64 contexts up to
 // 2048), 152 against 132 (256 of them).
