@@ -38,7 +38,7 @@ constexpr int kUnroll = 4;        // 16-byte pieces of a thread in a tile
 constexpr int kTile = kUnroll * 32, kTileBytes = kTile * 16;  // pieces and bytes of a warp's tile
 // Tiles of a warp under way, warps of a CTA that sum rows, that put results
 // together, and such CTAs an SM holds. 2048 rows of 32000 float32 took 47.8 us
-// with 2, 8, 2, 3 (now 50.8, 5.2 TB/s); with four tiles under way 54.9 (SMs
+// with 2, 8, 2, 3 (now 50.9, 5.2 TB/s); with four tiles under way 54.9 (SMs
 // drift apart: the rows are handed out beforehand), with one result warp 65.5,
 // with two CTAs of 8 + 2 or 8 + 4 warps 50.9 and 51.2, and 52 to 57 where all
 // warps of a CTA work on the results between rows.
@@ -170,7 +170,7 @@ struct Running {
 
   // The reference is the largest element so far: that element's term is exactly 1, no y is above 0, and log p and H
   // of a row with one likely token, differences of numbers as small as themselves, keep their signs and digits.
-  // (While it lagged by up to 20, both were off by 3e-6 there; 2048 rows of 32000 float32 took 49.5 us and take 50.8.)
+  // (While it lagged by up to 20, both were off by 3e-6 there; 2048 rows of 32000 float32 took 49.7 us and take 50.9.)
   TL_DEV void follow(float top) {
     if (top > m) {
       const float e = (m - top) * kLog2e, f = ex2(e);

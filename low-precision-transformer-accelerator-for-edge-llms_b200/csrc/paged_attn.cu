@@ -19,10 +19,11 @@
 //    has few rows, so a 128-row tcgen05 tile would be mostly padding and its
 //    result would have to come back through tensor memory; the 16-row tile is
 //    small enough to stay below the issue limit at full bandwidth.
-// Measured: one context of 131149 positions (bf16, 8 kv heads of 128) 90.3 us,
-// 5.9 TB/s; 16 contexts up to 8192 (float16) 50.7 us, 5.4 TB/s; 64 up to 2048
-// over INT8 (4 kv heads of 64) 18.6 us, 2.0 TB/s: 38 MB are too few to hide the
-// start (4 us), the joins (3 us) and the rounds' own chain (1.6 us each).
+// Measured: one context of 131149 positions (bf16, 8 kv heads of 128) 88.4 us,
+// 6.1 TB/s (94.0 with a float32 query, 83.5 with 4 kv heads of 16 query heads
+// each, 3.2 TB/s); 16 contexts up to 8192 (float16) 50.5 us, 5.4 TB/s; 64 up to
+// 2048 over INT8 (4 kv heads of 64) 17.6 us, 2.1 TB/s: 38 MB are too few to hide
+// the start (4 us), the joins (3 us) and the rounds' own chain (1.6 us each).
 //
 // Precision. Keys and values are exact, the other operand is split so that
 // nothing but its last bits is rounded; accumulators, maxima and sums are
@@ -36,7 +37,7 @@
 //    float32, of the probabilities always. With 16 bits of those, 15 and 26 of
 //    10000 bfloat16 outputs (17 and 5000 positions) were not the rounded
 //    float64 result, with 24 bits 1 and 7; one context of 131149 positions
-//    takes the same 89 us, 64 up to 2048 (4 kv heads of 64) 21.2 for 19.9.
+//    takes the same 89 us, 64 up to 2048 (4 kv heads of 64) 21.0 for 19.8.
 //  * Over an INT8 pool the query is a 22-bit integer times a power of two, as
 //    three signed digits to the base 256: two in the tile's rows, the third by
 //    a second MMA. Their sums are whole numbers. The probabilities are split as

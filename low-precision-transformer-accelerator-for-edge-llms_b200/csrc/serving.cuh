@@ -16,9 +16,9 @@ inline tl_status cuda_status(cudaError_t e) { return e == cudaSuccess ? TL_OK : 
 
 // Launches with programmatic serialization: a kernel's CTAs may be placed while
 // the kernel before it drains. Every thread of such a kernel calls pdl_begin()
-// before it touches global memory. Calls in a row, with and without: append of
-// 16 prompts 32.2 and 34.2 us, attention of 64 contexts over INT8 19.0 and
-// 20.5, log probabilities of 2048 rows 53.0 and 53.7.
+// before it touches global memory. Calls in a row, with and without, when it
+// came in: append of 16 prompts 32.2 and 34.2 us, attention of 64 contexts over
+// INT8 19.0 and 20.5, log probabilities of 2048 rows 53.0 and 53.7.
 template <typename... P, typename... A>
 tl_status launch_serving(void (*kernel)(P...), unsigned grid, int threads, size_t smem, int cluster, cudaStream_t s,
                          const A&... args) {
