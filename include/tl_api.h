@@ -617,18 +617,20 @@ TL_API tl_status tl_paged_read(const tl_paged_kv* cache, const tl_paged_read_arg
  * positions whose page does not exist are left out; a row without positions
  * (length 0, padding) gives zeros and lse = -infinity. Infinities in a 16-bit
  * pool (append rounds what a TL_F16 pool cannot hold to them) count as such: a
- * score of -infinity has weight 0 (a head left with nothing else gives zeros and
- * lse = -infinity), one of +infinity or NaN makes the head's out and lse NaN, as
- * does a NaN or an infinity in its query; an infinite value element gives its
- * infinity, NaN where both signs or a weight of 0 meet it (weights below 2^-33 of the
- * row's largest may count as 0 there). heads may be any multiple of kv_heads. Sums and softmax statistics are float32; products run
+ * score of -infinity has weight 0 (a head left with nothing else gives zeros
+ * and lse = -infinity), one of +infinity or NaN makes the head's out and lse
+ * NaN, as does a NaN or an infinity in its query; an infinite value element
+ * gives its infinity, NaN where both signs or a weight of 0 meet it (weights
+ * below 2^-33 of the row's largest may count as 0 there). heads may be any
+ * multiple of kv_heads. Sums and softmax statistics are float32; products run
  * on the tensor cores with the query and the probabilities split into parts of
  * fewer bits that add up to at least 22 of a float32 query's 24 bits (counted
  * from its row's largest element) and 24 (TL_BF16) or 22 of a probability's.
  * workspace: tl_paged_attn_workspace_bytes bytes of device memory, 16-byte
  * aligned, zeroed once by the caller before its first call; every call leaves
- * it ready for the next. Calls that share one workspace must not overlap on the GPU. The call
- * allocates nothing, does not synchronise and can be captured in a graph. */
+ * it ready for the next. Calls that share one workspace must not overlap on the
+ * GPU. The call allocates nothing, does not synchronise and can be captured in
+ * a graph. */
 TL_API size_t tl_paged_attn_workspace_bytes(int32_t heads, int32_t kv_heads, int32_t head_dim);
 typedef struct tl_paged_attn_args {
   const void* q;
